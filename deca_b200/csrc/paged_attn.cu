@@ -1,0 +1,76 @@
+// Entry points of the paged attention: argument rules, choice of the schedule, workspace.
+#include "paged_attn.cuh"
+
+namespace deca {
+size_t paged_rows_workspace(int D, int mt, int sms);
+int paged_rows_launch(int dtype, PagedArgs &g, int D, int mt, int sms, void *workspace, cudaStream_t st);
+
+namespace {
+
+bool tokens_ok(const deca_tokens &t) {
+    return aligned_to(t.data, 16) && t.token_stride % 8 == 0 && t.head_stride % 8 == 0;
+}
+bool cache_ok(const deca_cache &c) {
+    return aligned_to(c.data, 16) && c.page_stride % 8 == 0 && c.row_stride % 8 == 0 && c.head_stride % 8 == 0;
+}
+
+int row_tiles(const deca_paged_attn_args &a) { return (int64_t)a.max_q * (a.H_q / a.H_kv) <= 16 ? 1 : 2; }
+
+}  // namespace
+}  // namespace deca
+
+using namespace deca;
+
+extern "C" int deca_paged_attn_check(const deca_paged_attn_args *a) {
+    if (!a) return DECA_ERR_NULL;
+    if (a->dtype != DECA_F16 && a->dtype != DECA_BF16) return DECA_ERR_UNSUPPORTED;
+    if (a->D != 64 && a->D != 128) return DECA_ERR_UNSUPPORTED;
+    if (a->B < 1 || a->H_q < 1 || a->H_kv < 1 || a->H_q % a->H_kv != 0 || a->H_q / a->H_kv > 128) return DECA_ERR_SHAPE;
+    if (a->T < 0 || a->T > 2147483647ll || a->num_pages < 1 || a->num_pages > 2147483647ll) return DECA_ERR_SHAPE;
+    if (a->page_size != 16 && a->page_size != 32 && a->page_size != 64 && a->page_size != 128 && a->page_size != 256)
+        return DECA_ERR_SHAPE;
+    if (a->table_width < 1 || a->table_stride < a->table_width) return DECA_ERR_SHAPE;
+    if ((int64_t)a->table_width * a->page_size > 2147483647ll - 65536) return DECA_ERR_SHAPE;
+    if (a->max_q < 0 || a->max_kv < 0) return DECA_ERR_SHAPE;
+    if (!(a->scale == a->scale) || a->scale - a->scale != 0.f) return DECA_ERR_CONFIG;  // NaN or infinite
+    if (!a->Q.data || !a->O.data || !a->K.data || !a->V.data || !a->block_table || !a->cu_q || !a->kv_lens) return DECA_ERR_NULL;
+    if (!tokens_ok(a->Q) || !tokens_ok(a->O) || !cache_ok(a->K) || !cache_ok(a->V)) return DECA_ERR_ALIGN;
+    if (!aligned_to(a->block_table, 4) || !aligned_to(a->cu_q, 4) || !aligned_to(a->kv_lens, 4)) return DECA_ERR_ALIGN;
+    return DECA_OK;
+}
+
+extern "C" int deca_paged_attn_workspace_bytes(const deca_paged_attn_args *a, size_t *bytes) {
+    if (!a || !bytes) return DECA_ERR_NULL;
+    if ((a->D != 64 && a->D != 128) || a->H_kv < 1) return DECA_ERR_UNSUPPORTED;
+    DeviceInfo di;
+    if (int rc = current_device_info(&di)) return rc;
+    *bytes = paged_rows_workspace(a->D, row_tiles(*a), di.sms);
+    return DECA_OK;
+}
+
+extern "C" int deca_paged_attn(const deca_paged_attn_args *a, void *stream) {
+    if (int rc = deca_paged_attn_check(a)) return rc;
+    if (a->T == 0) return DECA_OK;
+    size_t need = 0;
+    if (int rc = deca_paged_attn_workspace_bytes(a, &need)) return rc;
+    if (!a->workspace) return DECA_ERR_NULL;
+    if (!aligned_to(a->workspace, 256)) return DECA_ERR_ALIGN;
+    if (a->workspace_bytes < need) return DECA_ERR_SCRATCH_LIMIT;
+    DeviceInfo di;
+    if (int rc = current_device_info(&di)) return rc;
+    PagedArgs g = {};
+    g.q = static_cast<const char *>(a->Q.data), g.q_st = a->Q.token_stride, g.q_sh = a->Q.head_stride;
+    g.o = static_cast<char *>(a->O.data), g.o_st = a->O.token_stride, g.o_sh = a->O.head_stride;
+    g.k = static_cast<const char *>(a->K.data), g.k_sp = a->K.page_stride, g.k_sr = a->K.row_stride, g.k_sh = a->K.head_stride;
+    g.v = static_cast<const char *>(a->V.data), g.v_sp = a->V.page_stride, g.v_sr = a->V.row_stride, g.v_sh = a->V.head_stride;
+    g.table = a->block_table, g.table_stride = a->table_stride, g.W = a->table_width;
+    g.cu = a->cu_q, g.kv_lens = a->kv_lens;
+    g.T = a->T, g.num_pages = a->num_pages, g.B = a->B, g.Hkv = a->H_kv, g.group = a->H_q / a->H_kv;
+    while ((1 << g.page_shift) < a->page_size) ++g.page_shift;
+    g.causal = a->causal ? 1 : 0;
+    g.sl2 = a->scale * kLog2e;
+    g.status = device_status_ptr();
+    if (!g.status) return (int)cudaErrorUnknown;
+    g.min_steps = 4;
+    return paged_rows_launch(a->dtype, g, a->D, row_tiles(*a), di.sms, a->workspace, static_cast<cudaStream_t>(stream));
+}

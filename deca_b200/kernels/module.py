@@ -24,7 +24,7 @@ SPEC_MAGIC = "deca_b200.kernel_spec.v1"
 
 @dataclass(frozen=True)
 class KernelSpec:
-    family: str  # "rowwise" | "gemm" | "flash_attn"
+    family: str  # "rowwise" | "gemm" | "flash_attn" | "add_rmsnorm" | "rotary" | "rotary_append" | "paged_step" | "paged_attn"
     shape: tuple
     dtype: str
     config: dict
@@ -67,19 +67,63 @@ def _check_tensor(t, shape, torch_dtype, name):
         raise ValueError(f"{name}: expected a contiguous tensor")
 
 
+def _check_view(t, shape, torch_dtype, name):
+    """A CUDA tensor on the current device whose last dimension is contiguous (other strides are free);
+    ``None`` in ``shape`` stands for any extent."""
+    ok = t.is_cuda and t.dtype == torch_dtype and len(t.shape) == len(shape)
+    if ok:
+        for have, want in zip(t.shape, shape):
+            ok = ok and (want is None or have == want)
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA tensor")
+    if not ok:
+        want = tuple("any" if d is None else d for d in shape)
+        raise ValueError(f"{name}: expected {torch_dtype} of shape {want}, got {t.dtype} of shape {tuple(t.shape)}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    _launch_device(t, name)
+
+
+def _launch_device(t, name):
+    """Kernels are launched on the current device's current stream, so tensors must live there; they
+    record no gradient, so a tensor that asks for one is refused."""
+    import torch
+
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name}: on cuda:{t.get_device()}, but the current device is cuda:{torch.cuda.current_device()}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name}: requires grad, but this operator records no gradient; call it under torch.no_grad()")
+
+
+@dataclass(frozen=True)
+class BuiltInSchedule:
+    """Config of an operator whose kernels choose their own launch shape: there is nothing to tune."""
+
+    def as_dict(self):
+        return {}
+
+    def __str__(self):
+        return "built-in schedule"
+
+
 class KernelModule:
     """A spec bound to the native library; ``module["main"]`` is the launch function."""
 
     entry_name = "main"
 
     def __init__(self, spec: KernelSpec):
-        from . import flash_attn_b200, gemm_b200, rowwise_b200
+        from . import add_rmsnorm_b200, flash_attn_b200, gemm_b200, paged_b200, rotary_b200, rowwise_b200
 
         self.spec = spec
         binder = {
             "rowwise": rowwise_b200.bind,
             "gemm": gemm_b200.bind,
             "flash_attn": flash_attn_b200.bind,
+            "add_rmsnorm": add_rmsnorm_b200.bind,
+            "rotary": rotary_b200.bind,
+            "rotary_append": rotary_b200.bind_append,
+            "paged_step": paged_b200.bind_step,
+            "paged_attn": paged_b200.bind_attn,
         }[spec.family]
         self._main = binder(spec)
 

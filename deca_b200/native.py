@@ -16,6 +16,8 @@ _lib = None
 F16, BF16 = 0, 1
 SOFTMAX, RMSNORM = 0, 1
 ROW_REG, ROW_TWOPASS, ROW_TMA, ROW_CLUSTER = 0, 1, 2, 3
+OUT_SAME, OUT_E4M3 = 0, 1
+ROT_HALF, ROT_INTERLEAVED = 0, 1
 DTYPE_CODE = {"float16": F16, "bfloat16": BF16}
 ROW_OP_CODE = {"softmax": SOFTMAX, "rmsnorm": RMSNORM}
 ROW_MODE_CODE = {"reg": ROW_REG, "twopass": ROW_TWOPASS, "tma": ROW_TMA, "cluster": ROW_CLUSTER}
@@ -48,6 +50,31 @@ class FaCfg(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in ("Br", "Bc", "stages", "q_tiles", "p_tmem", "persistent")]
 
 
+class Tokens(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class Cache(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
+class Rotation(ctypes.Structure):
+    _fields_ = [("D", ctypes.c_int), ("rot_dim", ctypes.c_int), ("layout", ctypes.c_int), ("inverse", ctypes.c_int),
+                ("amplitude", ctypes.c_float), ("turns", ctypes.POINTER(ctypes.c_uint64))]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    _fields_ = (
+        [(n, ctypes.c_int) for n in ("dtype", "B", "H_q", "H_kv", "D", "page_size", "causal")]
+        + [("scale", ctypes.c_float), ("T", ctypes.c_int64), ("num_pages", ctypes.c_int64),
+           ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int), ("max_q", ctypes.c_int),
+           ("max_kv", ctypes.c_int), ("Q", Tokens), ("O", Tokens), ("K", Cache), ("V", Cache)]
+        + [(n, ctypes.c_void_p) for n in ("block_table", "cu_q", "kv_lens", "workspace")]
+        + [("workspace_bytes", ctypes.c_size_t)]
+    )
+
+
 def lib() -> ctypes.CDLL:
     """The loaded library; raises if it has not been built."""
     global _lib
@@ -77,6 +104,14 @@ def lib() -> ctypes.CDLL:
         L.deca_fa_fwd_f16.argtypes = [vp, vp, vp, vp, ci, ci, ci, ci, ci, cf, ci, ctypes.POINTER(FaCfg), vp]
         L.deca_fa_fwd_f16_gather.argtypes = [vp, vp, vp, ctypes.POINTER(vp), ci, ci, ci, ci, ci, ci, ci, cf, ci,
                                              ctypes.POINTER(FaCfg), vp]
+        tp, cp, rp = ctypes.POINTER(Tokens), ctypes.POINTER(Cache), ctypes.POINTER(Rotation)
+        L.deca_add_rmsnorm.argtypes = [ci, vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, i64, cf, ci, ci, vp]
+        L.deca_rotary.argtypes = [ci, tp, tp, vp, i64, ci, rp, vp]
+        L.deca_rotary_append.argtypes = [ci, tp, tp, tp, tp, cp, cp, vp, vp, i64, ci, ci, i64, ci, rp, vp]
+        L.deca_paged_step.argtypes = [vp, vp, ci, vp, i64, ci, vp, ci, vp, ci, i64, vp, vp, vp, vp, vp, vp, vp]
+        L.deca_paged_attn_check.argtypes = [ctypes.POINTER(PagedAttnArgs)]
+        L.deca_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnArgs), ctypes.POINTER(ctypes.c_size_t)]
+        L.deca_paged_attn.argtypes = [ctypes.POINTER(PagedAttnArgs), vp]
         ip = ctypes.POINTER(ci)
         L.deca_last_device_status.argtypes = [ip, ip, ip, ci]
         L.deca_device_status_words.argtypes = [ctypes.POINTER(ctypes.c_uint), ci]

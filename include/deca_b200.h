@@ -254,6 +254,120 @@ int deca_fa_fwd_f16_gather(const void *Q, const void *K, const void *V, void *co
                            int B, int H, int S_q, int S_kv, int D, float softmax_scale, int causal,
                            const deca_fa_cfg *cfg, void *stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Residual addition + RMSNorm, the form RMSNorm takes between two layers:
+ *   H = dt(h),  h = X + R in fp32;   y = h * rsqrt(mean(h^2) + eps) * W in fp32 (h is not rounded
+ *   before it is normalised, and y is rounded once);   out = DECA_OUT_SAME: Y = dt(y), or
+ *   out = DECA_OUT_E4M3: Y = e4m3(y / s), s = max |y| / 448 over the row (group = 0) or over each
+ *   group of `group` (32, 64, 128 or 256) columns, the last one possibly short; scales[M, groups] fp32.
+ *   A scale below the smallest normal fp32 number (all of the group's y zero, in practice) gives zeros.
+ *   A NaN in a group makes its scale NaN.
+ * Row strides in elements, at least N; W contiguous.  Any N: rows that are no multiple of 8 elements
+ * or not 16-byte aligned take element-wise accesses.  H may be X or R itself, Y (of DECA_OUT_SAME) may
+ * be X; other overlaps are not allowed.  M = 0 launches nothing.
+ * No counterpart in the reference, whose RMSNorm has neither residual nor 8-bit output.
+ * ------------------------------------------------------------------------------------- */
+enum { DECA_OUT_SAME = 0, DECA_OUT_E4M3 = 1 };
+int deca_add_rmsnorm(int dtype, const void *X, int64_t x_stride, const void *R, int64_t r_stride, const void *W,
+                     void *H, int64_t h_stride, void *Y, int64_t y_stride, float *scales, int64_t M, int64_t N,
+                     float eps, int out, int group, void *stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Rotary positions.  Pair i of a head's first rot_dim elements turns by the angle
+ * 2 pi * position * turns[i] / 2^64:  (a, b) -> amplitude * (a cos - b sin, a sin + b cos).
+ * DECA_ROT_HALF pairs (i, i + rot_dim / 2), DECA_ROT_INTERLEAVED pairs (2i, 2i + 1); elements from
+ * rot_dim on are copied.  `turns` is a HOST array of rot_dim / 2 fixed-point fractions of a turn (it
+ * travels with the launch), so angles are exact modulo a turn at any position; inverse = 1 turns the
+ * other way, which is the transposed map, i.e. the gradient of the forward one.  fp32 arithmetic, one
+ * rounding.  D and rot_dim even, 2 <= rot_dim <= D <= 256.
+ * ------------------------------------------------------------------------------------- */
+enum { DECA_ROT_HALF = 0, DECA_ROT_INTERLEAVED = 1 };
+typedef struct {
+    void *data;           /* device pointer to [tokens, heads, D], innermost dimension contiguous */
+    int64_t token_stride; /* elements */
+    int64_t head_stride;
+} deca_tokens;
+typedef struct {
+    void *data; /* device pointer to [num_pages, page_size, H_kv, D], innermost dimension contiguous */
+    int64_t page_stride; /* elements */
+    int64_t row_stride;
+    int64_t head_stride;
+} deca_cache;
+typedef struct {
+    int D, rot_dim;
+    int layout;            /* DECA_ROT_HALF or DECA_ROT_INTERLEAVED */
+    int inverse;           /* 1: turn backwards */
+    float amplitude;       /* factor on cos and sin (1 unless the scaling method asks for one) */
+    const uint64_t *turns; /* host array, rot_dim / 2 entries */
+} deca_rotation;
+
+/* Y[t, h] = rotate(X[t, h], positions[t]); Y may be X itself (same pointer and strides). */
+int deca_rotary(int dtype, const deca_tokens *X, const deca_tokens *Y, const int32_t *positions, int64_t tokens,
+                int heads, const deca_rotation *rot, void *stream);
+
+/* Q_out = rotate(Q); row slots[t] of the cache = rotate(K[t]), V[t] in one launch, where slot s is row
+ * s % page_size of page s / page_size.  A slot outside [0, num_pages * page_size) writes nothing (padding
+ * rows carry -1); two tokens must not share a slot.  Q_out may be Q itself. */
+int deca_rotary_append(int dtype, const deca_tokens *Q, const deca_tokens *K, const deca_tokens *V,
+                       const deca_tokens *Q_out, const deca_cache *K_cache, const deca_cache *V_cache,
+                       const int32_t *positions, const int64_t *slots, int64_t tokens, int H_q, int H_kv,
+                       int64_t num_pages, int page_size, const deca_rotation *rot, void *stream);
+
+/* ---------------------------------------------------------------------------------------
+ * The bookkeeping of one serving step, on the device: from the cached length and the number of new
+ * tokens of every request,
+ *   cu_q[B + 1]   exclusive sum of new_lens;
+ *   kv_lens[B]    ctx_lens + new_lens (at most table_width * page_size);
+ *   block_table   entries ceil(ctx / page) .. ceil(kv / page) - 1 of every request take pages from the
+ *                 free list: the i-th page that the step needs, in request order, is
+ *                 free_pages[n_free - 1 - i] (-1 once the list is empty).  Other entries are left;
+ *   n_free_out    what the list still holds;  short_out: pages that were missing (0: none);
+ *   positions[T], slots[T]  of token t of the step: its place in its request, and
+ *                 page * page_size + row of the cache (-1 where it has no page).  Entries behind the last
+ *                 token get position 0 and slot -1; tokens beyond T are not written.
+ * Negative lengths count as 0.  Outputs must not overlap the inputs.  B <= 8192, page_size a power of two.
+ * ------------------------------------------------------------------------------------- */
+int deca_paged_step(const int32_t *ctx_lens, const int32_t *new_lens, int B, int32_t *block_table,
+                    int64_t table_stride, int table_width, const int32_t *free_pages, int free_capacity,
+                    const int32_t *n_free, int page_size, int64_t T, int32_t *cu_q, int32_t *kv_lens,
+                    int32_t *positions, int64_t *slots, int32_t *n_free_out, int32_t *short_out, void *stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Attention of new tokens over a paged cache: request r owns rows cu_q[r] .. cu_q[r + 1] - 1 of Q and O
+ * and the first kv_lens[r] rows of the pages block_table[r][0 ..]; its new tokens are the last of them.
+ * O[t, h] = softmax(scale * Q[t, h] K^T) V over the keys j <= kv_len - q_len + i (i = the token's place in
+ * its request; causal = 0: over all kv_len keys), key head h / (H_q / H_kv).  A row that sees no key is
+ * zero.  Rows of Q and O that belong to no request are not touched.  fp16 or bf16, fp32 scores, statistics
+ * and accumulators, D = 64 or 128, page_size 16, 32, 64, 128 or 256, H_q / H_kv <= 128.
+ * Lengths are read on the device and clipped to what T and the table hold; a table entry that names no
+ * page reads as zeros.  What a row cannot see never reaches it, whatever the cache holds there.
+ * max_q / max_kv: upper bounds of a request's new tokens and cached length as the caller knows them;
+ * they choose the schedule (any values give right results).
+ * ------------------------------------------------------------------------------------- */
+typedef struct {
+    int dtype;
+    int B;               /* requests */
+    int H_q, H_kv, D;
+    int page_size;
+    int causal;
+    float scale;
+    int64_t T;           /* rows of Q and O */
+    int64_t num_pages;
+    int64_t table_stride; /* elements */
+    int table_width;
+    int max_q, max_kv;
+    deca_tokens Q, O;
+    deca_cache K, V;
+    const int32_t *block_table, *cu_q, *kv_lens;
+    void *workspace;     /* deca_paged_attn_workspace_bytes, 256-byte aligned; contents need no preparation.
+                            Calls that overlap in time need one each */
+    size_t workspace_bytes;
+} deca_paged_attn_args;
+
+int deca_paged_attn_check(const deca_paged_attn_args *a);
+int deca_paged_attn_workspace_bytes(const deca_paged_attn_args *a, size_t *bytes);
+int deca_paged_attn(const deca_paged_attn_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
