@@ -4,6 +4,8 @@
 namespace deca {
 size_t paged_rows_workspace(int D, int mt, int sms);
 int paged_rows_launch(int dtype, PagedArgs &g, int D, int mt, int sms, void *workspace, cudaStream_t st);
+size_t paged_tiles_workspace(int D, int sms);
+int paged_tiles_launch(const deca_paged_attn_args &a, PagedArgs &g, int sms, cudaStream_t st);
 
 namespace {
 
@@ -14,7 +16,17 @@ bool cache_ok(const deca_cache &c) {
     return aligned_to(c.data, 16) && c.page_stride % 8 == 0 && c.row_stride % 8 == 0 && c.head_stride % 8 == 0;
 }
 
+// 16 rows each of the streaming schedule
 int row_tiles(const deca_paged_attn_args &a) { return (int64_t)a.max_q * (a.H_q / a.H_kv) <= 16 ? 1 : 2; }
+
+// The tensor-core tiles take what has more than 32 query rows per request and key head.
+bool use_tiles(const deca_paged_attn_args &a) {
+    return (int64_t)a.max_q * (a.H_q / a.H_kv) > 32 && a.scale > 0.f;  // the tiles keep maxima of unscaled scores
+}
+// ... and tensor maps want strides that advance
+bool strides_ok(const PagedArgs &g) {
+    return g.q_st > 0 && g.q_sh > 0 && g.k_sp > 0 && g.k_sr > 0 && g.k_sh > 0 && g.v_sp > 0 && g.v_sr > 0 && g.v_sh > 0;
+}
 
 }  // namespace
 }  // namespace deca
@@ -45,6 +57,7 @@ extern "C" int deca_paged_attn_workspace_bytes(const deca_paged_attn_args *a, si
     DeviceInfo di;
     if (int rc = current_device_info(&di)) return rc;
     *bytes = paged_rows_workspace(a->D, row_tiles(*a), di.sms);
+    if (use_tiles(*a) && paged_tiles_workspace(a->D, di.sms) > *bytes) *bytes = paged_tiles_workspace(a->D, di.sms);
     return DECA_OK;
 }
 
@@ -71,6 +84,10 @@ extern "C" int deca_paged_attn(const deca_paged_attn_args *a, void *stream) {
     g.sl2 = a->scale * kLog2e;
     g.status = device_status_ptr();
     if (!g.status) return (int)cudaErrorUnknown;
+    if (use_tiles(*a) && strides_ok(g)) {
+        g.min_steps = 2;
+        return paged_tiles_launch(*a, g, di.sms, static_cast<cudaStream_t>(stream));
+    }
     g.min_steps = 4;
     return paged_rows_launch(a->dtype, g, a->D, row_tiles(*a), di.sms, a->workspace, static_cast<cudaStream_t>(stream));
 }

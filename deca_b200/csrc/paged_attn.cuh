@@ -88,6 +88,33 @@ struct PackedRows {
     }
 };
 
+// Pairs of 128-row tiles of whole tokens (128 / group tokens each), KEYS keys per step.
+template <int KEYS>
+struct TokenTiles {
+    static constexpr int ROWS = 256;
+    static __device__ __forceinline__ int tokens(const PagedArgs &g) { return 128 / g.group; }  // of one of the two
+    static __device__ __forceinline__ bool place(const PagedArgs &g, const ReqView &v, int tile, int row, int &tok, int &j) {
+        const int r = row & 127, t = r / g.group, n = tokens(g);
+        tok = (2 * tile + (row >> 7)) * n + t;
+        j = r - t * g.group;
+        return t < n && tok < v.n;
+    }
+    static __device__ __forceinline__ int tiles(const PagedArgs &g, const ReqView &v) {
+        const int n = 2 * tokens(g);
+        return (v.n + n - 1) / n;
+    }
+    static __device__ __forceinline__ int steps(const PagedArgs &g, const ReqView &v, int tile) {
+        const int last = min((tile + 1) * 2 * tokens(g), v.n) - 1;
+        return max((keys_until(v, last) + KEYS - 1) / KEYS, 1);
+    }
+    static __device__ __forceinline__ long long head_steps(const PagedArgs &g, const ReqView &v) {
+        long long s = 0;
+        const int n = tiles(g, v);
+        for (int t = 0; t < n; ++t) s += steps(g, v, t);
+        return s;
+    }
+};
+
 // A CTA's place in the list of items.
 struct WorkPos {
     int req, head, tile;

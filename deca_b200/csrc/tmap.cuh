@@ -29,7 +29,7 @@ inline EncodeTiledFn encode_tiled_fn() {
     return fn;
 }
 
-// 16-bit row-major tensor of up to 3 dimensions, innermost first in `dims` / `box`;
+// 16-bit row-major tensor of up to 4 dimensions, innermost first in `dims` / `box`;
 // `strides_bytes` holds the pitch of dimensions 1..rank-1.  Out-of-bounds reads give zero.
 // Returns 0 or a positive error code.
 inline int make_tmap_16bit(CUtensorMap *out, int dtype, const void *base, int rank, const uint64_t *dims,
@@ -39,8 +39,8 @@ inline int make_tmap_16bit(CUtensorMap *out, int dtype, const void *base, int ra
     // the launch path.
     struct Key {
         const void *base;
-        uint64_t dims[3], strides[2];
-        uint32_t box[3];
+        uint64_t dims[4], strides[3];
+        uint32_t box[4];
         int dtype, rank, swizzle;
     };
     struct Entry {
@@ -65,9 +65,9 @@ inline int make_tmap_16bit(CUtensorMap *out, int dtype, const void *base, int ra
         }
     EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return (int)cudaErrorSymbolNotFound;
-    cuuint64_t gdim[3];
-    cuuint64_t gstr[2];
-    cuuint32_t bx[3], es[3];
+    cuuint64_t gdim[4];
+    cuuint64_t gstr[3];
+    cuuint32_t bx[4], es[4];
     for (int i = 0; i < rank; ++i) {
         gdim[i] = dims[i];
         bx[i] = box[i];
