@@ -1,4 +1,5 @@
-"""Builds libdeca_b200.so (the C-ABI library of sm_100a kernels) in-tree with nvcc.
+"""Builds libdeca_b200.so (the C-ABI library of sm_100a kernels) in-tree with nvcc, and _launch.so (the
+CPython extension that checks and launches the serving operators on torch tensors) with g++.
 
     python -m deca_b200.build [--force] [--verbose]
 
@@ -21,6 +22,8 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 OBJ_DIR = os.path.join(PKG, "build")
 LIB_PATH = os.path.join(PKG, "libdeca_b200.so")
+LAUNCH_SRC = os.path.join(CSRC, "launch.cpp")
+LAUNCH_PATH = os.path.join(PKG, "_launch.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -38,11 +41,37 @@ def _headers():
     return sorted(glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h")))
 
 
-def is_up_to_date() -> bool:
-    if not os.path.exists(LIB_PATH):
+def _newer(target: str, sources) -> bool:
+    if not os.path.exists(target):
         return False
-    t = os.path.getmtime(LIB_PATH)
-    return all(os.path.getmtime(p) <= t for p in _sources() + _headers() + [os.path.abspath(__file__)])
+    t = os.path.getmtime(target)
+    return all(os.path.getmtime(p) <= t for p in sources)
+
+
+def is_up_to_date() -> bool:
+    return _newer(LIB_PATH, _sources() + _headers() + [os.path.abspath(__file__)])
+
+
+def build_launch(force: bool = False) -> str:
+    """Compiles the extension against torch's headers; it finds the library beside itself."""
+    header = os.path.join(INCLUDE, "deca_b200.h")
+    if not force and _newer(LAUNCH_PATH, [LAUNCH_SRC, header, os.path.abspath(__file__)]):
+        return LAUNCH_PATH
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    includes = [INCLUDE, os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{p}" for p in includes], LAUNCH_SRC, "-o", LAUNCH_PATH, "-L" + os.path.join(root, "lib"), "-L" + PKG,
+           "-l:libdeca_b200.so", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {LAUNCH_SRC}:\n{res.stderr[-4000:]}")
+    return LAUNCH_PATH
 
 
 def _compile(src: str, verbose: bool) -> str:
@@ -60,8 +89,10 @@ def _compile(src: str, verbose: bool) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compiles every CUDA source for sm_100a and links the shared library; returns its path."""
+    """Compiles every CUDA source for sm_100a and links the shared library, then the launch extension;
+    returns the library's path."""
     if not force and is_up_to_date():
+        build_launch()
         return LIB_PATH
     os.makedirs(OBJ_DIR, exist_ok=True)
     if force:
@@ -74,6 +105,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stderr[-4000:]}")
+    build_launch(force)
     return LIB_PATH
 
 

@@ -3,17 +3,20 @@
 //   h = x + res;  y = h * rsqrt(sum h^2 / N + eps) * w;  out dt(h) and dt(y), or e4m3(y / s) with
 //   s = max |y| / 448 over the row or a group of columns.
 //
-// One pass: a row's h stays in fp32 registers between the sum of squares and the output (8 elements
-// per chunk, C chunks per thread), so every element is read once and written once, which is the floor
-// of an HBM-bound operator: 8 bytes per element, 7 with the 8-bit output.  The row is spread over
-// threads in interleaved 16-byte chunks as in rowwise.cu; the columns of a scale group (a multiple of 32)
-// are then the chunks of 4 .. 32 neighbouring lanes, whose maximum takes shuffles alone.
+// One pass: a row's h stays in fp32 registers between the sum of squares and the output, so every element
+// is read once and written once, which is the floor of an HBM-bound operator: 8 bytes per element, 7
+// with the 8-bit output.  A warp takes spans of 256 columns, eight per lane, in accesses of V elements: V =
+// 8 (16 bytes) where rows are aligned, else 4, 2 or 1, with the lanes of one access side by side, so that
+// an odd row length costs instructions but not sectors.  The columns of a scale group (32 .. 256) then lie
+// in one warp's span and its maximum takes shuffles alone.
 // Rows beyond the registers of a CTA are streamed twice (three times for one scale a row).
 #include "common.cuh"
 
 namespace deca {
 namespace {
 
+constexpr int kMaxRegThreads = 512;
+constexpr int kGrouped = 2;  // DECA_OUT_E4M3 with a scale per group of columns
 constexpr float kE4m3Max = 448.0f;
 constexpr float kMinScale = 1.17549435e-38f;  // below it 1 / s is no finite number: the group is written as zeros
 
@@ -25,7 +28,7 @@ struct AddNormArgs {
     long long sx, sr, sh, sy;  // row strides in elements
     int N;
     int tpr;  // threads per row
-    int group, n_groups;
+    int group_shift, n_groups;  // log2 of a scale group's columns (0: one scale a row)
     float eps, inv_n;
 };
 
@@ -48,42 +51,64 @@ __device__ __forceinline__ void store1(char *p, float v) {
         *reinterpret_cast<__nv_bfloat16 *>(p) = __float2bfloat16_rn(v);
 }
 
-// Eight consecutive elements from column `col` on as fp32; element-wise with zeros behind the row's end
-// where rows are not made of aligned 16-byte chunks.
-template <int DT, bool VEC>
-__device__ __forceinline__ void load8(float (&f)[8], const char *row, int col, int N, bool stream) {
-    if constexpr (VEC) {
-        uint32_t d[4];
-        if (stream)
-            asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                         : "l"(row + (size_t)col * 2));
-        else
-            asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                         : "l"(row + (size_t)col * 2));
+// Column of element i (0 .. 7) of a lane in the span that starts at `span`: access i / V, V elements each.
+template <int V>
+__device__ __forceinline__ int column(int span, int lane, int i) {
+    return span + (i / V) * 32 * V + lane * V + i % V;
+}
+
+// A lane's eight elements of a span as fp32, zeros behind the row's end (N is a multiple of V).
+template <int DT, int V, bool STREAM>
+__device__ __forceinline__ void load8(float (&f)[8], const char *row, int span, int lane, int N) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 v = Pack16<DT>::unpack(d[i]);
-            f[2 * i] = v.x, f[2 * i + 1] = v.y;
+    for (int a = 0; a < 8; a += V) {
+        const int col = column<V>(span, lane, a);
+        const char *p = row + (size_t)col * 2;
+        if constexpr (V == 1) {
+            f[a] = col < N ? load1<DT>(p) : 0.f;
+        } else {
+            uint32_t d[V / 2];
+#pragma unroll
+            for (int k = 0; k < V / 2; ++k) d[k] = 0u;
+            if (col < N) {
+                if constexpr (V == 8 && STREAM)
+                    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                                 : "l"(p));
+                else if constexpr (V == 8)
+                    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "l"(p));
+                else if constexpr (V == 4)
+                    asm volatile("ld.global.v2.u32 {%0,%1}, [%2];" : "=r"(d[0]), "=r"(d[1]) : "l"(p));
+                else
+                    asm volatile("ld.global.u32 %0, [%1];" : "=r"(d[0]) : "l"(p));
+            }
+#pragma unroll
+            for (int k = 0; k < V / 2; ++k) {
+                const float2 v = Pack16<DT>::unpack(d[k]);
+                f[a + 2 * k] = v.x, f[a + 2 * k + 1] = v.y;
+            }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = col + i < N ? load1<DT>(row + (size_t)(col + i) * 2) : 0.f;
     }
 }
 
-template <int DT, bool VEC>
-__device__ __forceinline__ void store8(char *row, int col, int N, const float (&f)[8]) {
-    if constexpr (VEC) {
-        asm volatile("st.global.cs.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(row + (size_t)col * 2),
-                     "r"(Pack16<DT>::pack(f[0], f[1])), "r"(Pack16<DT>::pack(f[2], f[3])),
-                     "r"(Pack16<DT>::pack(f[4], f[5])), "r"(Pack16<DT>::pack(f[6], f[7]))
-                     : "memory");
-    } else {
+template <int DT, int V>
+__device__ __forceinline__ void store8(char *row, int span, int lane, int N, const float (&f)[8]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (col + i < N) store1<DT>(row + (size_t)(col + i) * 2, f[i]);
+    for (int a = 0; a < 8; a += V) {
+        const int col = column<V>(span, lane, a);
+        char *p = row + (size_t)col * 2;
+        if (col >= N) continue;
+        if constexpr (V == 1) {
+            store1<DT>(p, f[a]);
+        } else if constexpr (V == 8) {
+            asm volatile("st.global.cs.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(Pack16<DT>::pack(f[0], f[1])),
+                         "r"(Pack16<DT>::pack(f[2], f[3])), "r"(Pack16<DT>::pack(f[4], f[5])), "r"(Pack16<DT>::pack(f[6], f[7]))
+                         : "memory");
+        } else if constexpr (V == 4) {
+            *reinterpret_cast<uint2 *>(p) = make_uint2(Pack16<DT>::pack(f[a], f[a + 1]), Pack16<DT>::pack(f[a + 2], f[a + 3]));
+        } else {
+            *reinterpret_cast<uint32_t *>(p) = Pack16<DT>::pack(f[a], f[a + 1]);
+        }
     }
 }
 
@@ -94,16 +119,25 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return v;
 }
 
-template <bool VEC>
-__device__ __forceinline__ void store_e4m3(char *row, int col, int N, const float (&y)[8], float inv) {
-    uint32_t lo = e4m3x2(y[0] * inv, y[1] * inv) | (e4m3x2(y[2] * inv, y[3] * inv) << 16);
-    uint32_t hi = e4m3x2(y[4] * inv, y[5] * inv) | (e4m3x2(y[6] * inv, y[7] * inv) << 16);
-    if constexpr (VEC) {
-        asm volatile("st.global.cs.v2.u32 [%0], {%1,%2};" ::"l"(row + col), "r"(lo), "r"(hi) : "memory");
-    } else {
+template <int V>
+__device__ __forceinline__ void store_e4m3(char *row, int span, int lane, int N, const float (&y)[8], const float (&inv)[8 / V]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (col + i < N) row[col + i] = (char)(((i < 4 ? lo : hi) >> (8 * (i & 3))) & 0xFFu);
+    for (int a = 0; a < 8; a += V) {
+        const int col = column<V>(span, lane, a);
+        const float s = inv[a / V];
+        if (col >= N) continue;
+        if constexpr (V == 8)
+            asm volatile("st.global.cs.v2.u32 [%0], {%1,%2};" ::"l"(row + col),
+                         "r"(e4m3x2(y[0] * s, y[1] * s) | (e4m3x2(y[2] * s, y[3] * s) << 16)),
+                         "r"(e4m3x2(y[4] * s, y[5] * s) | (e4m3x2(y[6] * s, y[7] * s) << 16))
+                         : "memory");
+        else if constexpr (V == 4)
+            *reinterpret_cast<uint32_t *>(row + col) =
+                e4m3x2(y[a] * s, y[a + 1] * s) | (e4m3x2(y[a + 2] * s, y[a + 3] * s) << 16);
+        else if constexpr (V == 2)
+            *reinterpret_cast<uint16_t *>(row + col) = (uint16_t)e4m3x2(y[a] * s, y[a + 1] * s);
+        else
+            row[col] = (char)(e4m3x2(y[a] * s, 0.f) & 0xFFu);
     }
 }
 
@@ -117,22 +151,48 @@ __device__ __forceinline__ float abs_max8(const float (&y)[8]) {
 // Scale and its inverse of a group whose largest |y| is `m`.
 __device__ __forceinline__ void scale_of(float m, float &s, float &inv) {
     s = m * (1.0f / kE4m3Max);
-    inv = s >= kMinScale ? 1.0f / s : 0.f;
+    inv = s >= kMinScale ? __frcp_rn(s) : 0.f;
 }
 
-// One chunk of a grouped e4m3 output: maximum over the lanes that share the group, scale, store.
-// Called by all lanes of a warp; `col` is ordered by lane and group / 8 lanes share a group.
-template <bool VEC>
-__device__ __forceinline__ void store_grouped(const AddNormArgs &a, long long row, char *yrow, int col, bool live,
-                                              const float (&y)[8]) {
-    float m = live ? abs_max8(y) : 0.f;
-    for (int s = a.group >> 4; s >= 1; s >>= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, s));
-    float scale, inv;
-    scale_of(m, scale, inv);
-    if (live) {
-        if (col % a.group == 0) a.scales[row * a.n_groups + col / a.group] = scale;
-        store_e4m3<VEC>(yrow, col, a.N, y, inv);
+// A span of a grouped e4m3 output: maxima over the lanes (and accesses) that share a group, scales, store.
+// Called by all lanes of a warp, with y = 0 behind the row's end.
+template <int V>
+__device__ __forceinline__ void store_grouped(const AddNormArgs &a, long long row, char *yrow, int span, int lane, const float (&y)[8]) {
+    constexpr int A = 8 / V;  // accesses
+    float m[A], inv[A];
+#pragma unroll
+    for (int k = 0; k < A; ++k) {
+        m[k] = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) m[k] = max_nan(m[k], fabsf(y[k * V + i]));
     }
+    const int group = 1 << a.group_shift;
+    // groups wider than an access of the warp (32 V columns): neighbouring accesses share a maximum
+#pragma unroll
+    for (int w = 1; w < A; w *= 2)
+        if (group >= 64 * V * w) {
+#pragma unroll
+            for (int k = 0; k < A; k += 2 * w) {
+                float t = max_nan(m[k], m[k + w]);
+#pragma unroll
+                for (int i = 0; i < 2 * w; ++i) m[k + i] = t;
+            }
+        }
+    const int lanes = min(group / V, 32);
+#pragma unroll
+    for (int s = 16; s >= 1; s >>= 1)
+        if (s < lanes) {
+#pragma unroll
+            for (int k = 0; k < A; ++k) m[k] = max_nan(m[k], __shfl_xor_sync(0xFFFFFFFFu, m[k], s));
+        }
+#pragma unroll
+    for (int k = 0; k < A; ++k) {
+        float scale;
+        scale_of(m[k], scale, inv[k]);
+        const int col = column<V>(span, lane, k * V);
+        if ((col & (group - 1)) == 0 && col < a.N) a.scales[row * a.n_groups + (col >> a.group_shift)] = scale;
+    }
+    store_e4m3<V>(yrow, span, lane, a.N, y, inv);
 }
 
 template <bool MAX>
@@ -151,34 +211,30 @@ __device__ __forceinline__ float row_reduce(float v, float *red, int nw, int row
     return v;
 }
 
-// The row in registers: C chunks of eight elements per thread, `rpb` rows per CTA.
-template <int DT, int OUT, int C, bool VEC>
-__global__ void add_rmsnorm_reg_kernel(const AddNormArgs a) {
+// The row in registers: C spans per warp, `rpb` rows per CTA.  OUT: DECA_OUT_SAME, DECA_OUT_E4M3 (one scale a
+// row) or kGrouped.
+template <int DT, int OUT, int C, int V>
+__global__ void __launch_bounds__(kMaxRegThreads) add_rmsnorm_reg_kernel(const AddNormArgs a) {
     __shared__ float red[2][32];
     const int t = threadIdx.x % a.tpr, rb = threadIdx.x / a.tpr;
     const int lane = threadIdx.x & 31, wr = t >> 5, nw = a.tpr >> 5;
-    long long row = (long long)blockIdx.x * (blockDim.x / a.tpr) + rb;
-    const bool live_row = row < a.M;  // the threads of a row behind the last one take part in the barriers only
-    if (!live_row) row = 0;
+    const long long row = (long long)blockIdx.x * (blockDim.x / a.tpr) + rb;
+    const bool live = row < a.M;  // the threads of a row behind the last one take part in the barriers only
+    const int N = live ? a.N : 0;
     const char *xrow = a.x + row * a.sx * 2, *rrow = a.r + row * a.sr * 2;
     char *hrow = a.h + row * a.sh * 2, *yrow = a.y + row * a.sy * (OUT == DECA_OUT_SAME ? 2 : 1);
 
     float h[C][8];
-    float ss = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        const int col = (c * a.tpr + t) * 8;
+        const int span = (c * nw + wr) * 256;
         float r[8];
-        if (live_row && col < a.N) {
-            load8<DT, VEC>(h[c], xrow, col, a.N, true);
-            load8<DT, VEC>(r, rrow, col, a.N, true);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) h[c][i] = r[i] = 0.f;
-        }
+        load8<DT, V, true>(h[c], xrow, span, lane, N);
+        load8<DT, V, true>(r, rrow, span, lane, N);
 #pragma unroll
         for (int i = 0; i < 8; ++i) h[c][i] += r[i];
     }
+    float ss = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -189,139 +245,129 @@ __global__ void add_rmsnorm_reg_kernel(const AddNormArgs a) {
     float amax = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        const int col = (c * a.tpr + t) * 8;
-        const bool live = live_row && col < a.N;
-        if (live) store8<DT, VEC>(hrow, col, a.N, h[c]);
+        const int span = (c * nw + wr) * 256;
+        store8<DT, V>(hrow, span, lane, N, h[c]);
         float w[8];
-        if (live) {
-            load8<DT, VEC>(w, a.w, col, a.N, false);
+        load8<DT, V, false>(w, a.w, span, lane, N);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[c][i] = h[c][i] * rs * w[i];
-        }
-        if constexpr (OUT == DECA_OUT_SAME) {
-            if (live) store8<DT, VEC>(yrow, col, a.N, h[c]);
-        } else if (a.group > 0) {
-            store_grouped<VEC>(a, row, yrow, col, live, h[c]);
-        } else if (live) {
+        for (int i = 0; i < 8; ++i) h[c][i] = h[c][i] * rs * w[i];
+        if constexpr (OUT == DECA_OUT_SAME)
+            store8<DT, V>(yrow, span, lane, N, h[c]);
+        else if constexpr (OUT == DECA_OUT_E4M3)
             amax = max_nan(amax, abs_max8(h[c]));
-        }
+        else if (live && span < N)
+            store_grouped<V>(a, row, yrow, span, lane, h[c]);
     }
     if constexpr (OUT == DECA_OUT_E4M3) {
-        if (a.group == 0) {
-            amax = row_reduce<true>(amax, red[1], nw, rb * nw, wr, lane);
-            float scale, inv;
-            scale_of(amax, scale, inv);
-            if (live_row && t == 0) a.scales[row] = scale;
+        amax = row_reduce<true>(amax, red[1], nw, rb * nw, wr, lane);
+        float scale, inv1, inv[8 / V];
+        scale_of(amax, scale, inv1);
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int col = (c * a.tpr + t) * 8;
-                if (live_row && col < a.N) store_e4m3<VEC>(yrow, col, a.N, h[c], inv);
-            }
-        }
+        for (int k = 0; k < 8 / V; ++k) inv[k] = inv1;
+        if (live && t == 0) a.scales[row] = scale;
+#pragma unroll
+        for (int c = 0; c < C; ++c) store_e4m3<V>(yrow, (c * nw + wr) * 256, lane, N, h[c], inv);
     }
 }
 
 // Rows of any length: the row is read once for the sum of squares, (one scale a row) once for the
 // maximum and once for the output; re-reads come from L2.
-template <int DT, int OUT, bool VEC>
-__global__ void add_rmsnorm_stream_kernel(const AddNormArgs a) {
+template <int DT, int OUT, int V>
+__global__ void __launch_bounds__(kMaxRegThreads) add_rmsnorm_stream_kernel(const AddNormArgs a) {
     __shared__ float red[2][32];
     const int t = threadIdx.x, lane = t & 31, wr = t >> 5, nw = blockDim.x >> 5;
     const long long row = blockIdx.x;
     const char *xrow = a.x + row * a.sx * 2, *rrow = a.r + row * a.sr * 2;
     char *hrow = a.h + row * a.sh * 2, *yrow = a.y + row * a.sy * (OUT == DECA_OUT_SAME ? 2 : 1);
-    const int span = (int)blockDim.x * 8;
-    auto load_h = [&](float (&h)[8], int col) {
+    const int step = nw * 256, first = wr * 256;
+    auto load_h = [&](float (&h)[8], int span) {
         float r[8];
-        load8<DT, VEC>(h, xrow, col, a.N, false);
-        load8<DT, VEC>(r, rrow, col, a.N, false);
+        load8<DT, V, false>(h, xrow, span, lane, a.N);
+        load8<DT, V, false>(r, rrow, span, lane, a.N);
 #pragma unroll
         for (int i = 0; i < 8; ++i) h[i] += r[i];
     };
-    auto load_y = [&](float (&y)[8], int col, float rs) {
+    auto scale_h = [&](float (&y)[8], int span, float rs) {
         float w[8];
-        load8<DT, VEC>(w, a.w, col, a.N, false);
+        load8<DT, V, false>(w, a.w, span, lane, a.N);
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = y[i] * rs * w[i];
     };
     float ss = 0.f;
-    for (int base = 0; base < a.N; base += span) {
-        const int col = base + t * 8;
-        if (col < a.N) {
-            float h[8];
-            load_h(h, col);
+    for (int span = first; span < a.N; span += step) {
+        float h[8];
+        load_h(h, span);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss = fmaf(h[i], h[i], ss);
-        }
+        for (int i = 0; i < 8; ++i) ss = fmaf(h[i], h[i], ss);
     }
     ss = row_reduce<false>(ss, red[0], nw, 0, wr, lane);
     const float rs = rsqrtf(fmaf(ss, a.inv_n, a.eps));
-    float scale = 0.f, inv = 0.f;
+    float inv[8 / V];
     if constexpr (OUT == DECA_OUT_E4M3) {
-        if (a.group == 0) {
-            float amax = 0.f;
-            for (int base = 0; base < a.N; base += span) {
-                const int col = base + t * 8;
-                if (col < a.N) {
-                    float y[8];
-                    load_h(y, col);
-                    load_y(y, col, rs);
-                    amax = max_nan(amax, abs_max8(y));
-                }
-            }
-            amax = row_reduce<true>(amax, red[1], nw, 0, wr, lane);
-            scale_of(amax, scale, inv);
-            if (t == 0) a.scales[row] = scale;
+        float amax = 0.f;
+        for (int span = first; span < a.N; span += step) {
+            float y[8];
+            load_h(y, span);
+            scale_h(y, span, rs);
+            amax = max_nan(amax, abs_max8(y));
         }
+        amax = row_reduce<true>(amax, red[1], nw, 0, wr, lane);
+        float scale, inv1;
+        scale_of(amax, scale, inv1);
+#pragma unroll
+        for (int k = 0; k < 8 / V; ++k) inv[k] = inv1;
+        if (t == 0) a.scales[row] = scale;
     }
     // every element is read again and then written by the same thread, so H may be X or R
-    for (int base = 0; base < a.N; base += span) {
-        const int col = base + t * 8;
-        const bool live = col < a.N;
-        float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (live) {
-            load_h(y, col);
-            store8<DT, VEC>(hrow, col, a.N, y);
-            load_y(y, col, rs);
-        }
-        if constexpr (OUT == DECA_OUT_SAME) {
-            if (live) store8<DT, VEC>(yrow, col, a.N, y);
-        } else if (a.group > 0) {
-            store_grouped<VEC>(a, row, yrow, col, live, y);
-        } else if (live) {
-            store_e4m3<VEC>(yrow, col, a.N, y, inv);
-        }
+    for (int span = first; span < a.N; span += step) {
+        float y[8];
+        load_h(y, span);
+        store8<DT, V>(hrow, span, lane, a.N, y);
+        scale_h(y, span, rs);
+        if constexpr (OUT == DECA_OUT_SAME)
+            store8<DT, V>(yrow, span, lane, a.N, y);
+        else if constexpr (OUT == DECA_OUT_E4M3)
+            store_e4m3<V>(yrow, span, lane, a.N, y, inv);
+        else
+            store_grouped<V>(a, row, yrow, span, lane, y);
     }
 }
 
-constexpr int kMaxChunks = 8;
-constexpr int kMaxRegThreads = 512;
-
-template <int DT, int OUT, bool VEC>
-int launch(const AddNormArgs &a0, int chunks, int rpb, cudaStream_t st) {
-    AddNormArgs a = a0;
-    if (chunks == 0) {
+template <int DT, int OUT, int V>
+int launch(const AddNormArgs &a, int spans, int rpb, cudaStream_t st) {
+    if (spans == 0) {
         if (a.M > 2147483647ll) return DECA_ERR_SHAPE;
-        add_rmsnorm_stream_kernel<DT, OUT, VEC><<<(unsigned)a.M, 512, 0, st>>>(a);
+        add_rmsnorm_stream_kernel<DT, OUT, V><<<(unsigned)a.M, 512, 0, st>>>(a);
         return (int)cudaGetLastError();
     }
     const long long grid = (a.M + rpb - 1) / rpb;
     if (grid > 2147483647ll) return DECA_ERR_SHAPE;
     const unsigned g = (unsigned)grid, threads = (unsigned)(a.tpr * rpb);
-    switch (chunks) {
-        case 1: add_rmsnorm_reg_kernel<DT, OUT, 1, VEC><<<g, threads, 0, st>>>(a); break;
-        case 2: add_rmsnorm_reg_kernel<DT, OUT, 2, VEC><<<g, threads, 0, st>>>(a); break;
-        case 4: add_rmsnorm_reg_kernel<DT, OUT, 4, VEC><<<g, threads, 0, st>>>(a); break;
-        default: add_rmsnorm_reg_kernel<DT, OUT, 8, VEC><<<g, threads, 0, st>>>(a); break;
+    switch (spans) {
+        case 1: add_rmsnorm_reg_kernel<DT, OUT, 1, V><<<g, threads, 0, st>>>(a); break;
+        case 2: add_rmsnorm_reg_kernel<DT, OUT, 2, V><<<g, threads, 0, st>>>(a); break;
+        case 3: add_rmsnorm_reg_kernel<DT, OUT, 3, V><<<g, threads, 0, st>>>(a); break;
+        case 4: add_rmsnorm_reg_kernel<DT, OUT, 4, V><<<g, threads, 0, st>>>(a); break;
+        default: add_rmsnorm_reg_kernel<DT, OUT, 8, V><<<g, threads, 0, st>>>(a); break;
     }
     return (int)cudaGetLastError();
 }
 
+template <int DT, int OUT>
+int launch_width(const AddNormArgs &a, int v, int spans, int rpb, cudaStream_t st) {
+    switch (v) {
+        case 8: return launch<DT, OUT, 8>(a, spans, rpb, st);
+        case 4: return launch<DT, OUT, 4>(a, spans, rpb, st);
+        case 2: return launch<DT, OUT, 2>(a, spans, rpb, st);
+        default: return launch<DT, OUT, 1>(a, spans, rpb, st);
+    }
+}
+
 template <int DT>
-int launch_out(const AddNormArgs &a, int out, bool vec, int chunks, int rpb, cudaStream_t st) {
-    if (out == DECA_OUT_SAME)
-        return vec ? launch<DT, DECA_OUT_SAME, true>(a, chunks, rpb, st) : launch<DT, DECA_OUT_SAME, false>(a, chunks, rpb, st);
-    return vec ? launch<DT, DECA_OUT_E4M3, true>(a, chunks, rpb, st) : launch<DT, DECA_OUT_E4M3, false>(a, chunks, rpb, st);
+int launch_out(const AddNormArgs &a, int out, int v, int spans, int rpb, cudaStream_t st) {
+    if (out == DECA_OUT_SAME) return launch_width<DT, DECA_OUT_SAME>(a, v, spans, rpb, st);
+    return a.group_shift > 0 ? launch_width<DT, kGrouped>(a, v, spans, rpb, st)
+                             : launch_width<DT, DECA_OUT_E4M3>(a, v, spans, rpb, st);
 }
 
 }  // namespace
@@ -344,28 +390,36 @@ extern "C" int deca_add_rmsnorm(int dtype, const void *X, int64_t x_stride, cons
     if (!aligned_to(X, 2) || !aligned_to(R, 2) || !aligned_to(W, 2) || !aligned_to(H, 2) || !aligned_to(Y, out_bytes) ||
         !aligned_to(scales, 4))
         return DECA_ERR_ALIGN;
-    const bool rows_vec = M == 1 || (x_stride % 8 == 0 && r_stride % 8 == 0 && h_stride % 8 == 0 && y_stride % 8 == 0);
-    const bool vec = N % 8 == 0 && rows_vec && aligned_to(X, 16) && aligned_to(R, 16) && aligned_to(W, 16) &&
-                     aligned_to(H, 16) && aligned_to(Y, 8 * out_bytes);
+    // elements per access: the widest that the row length, the strides and the bases allow
+    int v = 8;
+    auto fits = [&](int w) {
+        const bool strides = M == 1 || (x_stride % w == 0 && r_stride % w == 0 && h_stride % w == 0 && y_stride % w == 0);
+        return N % w == 0 && strides && aligned_to(X, 2 * w) && aligned_to(R, 2 * w) && aligned_to(W, 2 * w) &&
+               aligned_to(H, 2 * w) && aligned_to(Y, w * out_bytes);
+    };
+    while (v > 1 && !fits(v)) v /= 2;
     AddNormArgs a;
     a.x = static_cast<const char *>(X), a.r = static_cast<const char *>(R), a.w = static_cast<const char *>(W);
     a.h = static_cast<char *>(H), a.y = static_cast<char *>(Y), a.scales = scales;
     a.M = M, a.N = (int)N;
     a.sx = x_stride, a.sr = r_stride, a.sh = h_stride, a.sy = y_stride;
-    a.group = group;
+    a.group_shift = 0;
+    while (group && (1 << a.group_shift) < group) ++a.group_shift;
     a.n_groups = group ? (int)((N + group - 1) / group) : 1;
     a.eps = eps, a.inv_n = 1.0f / (float)N;
-    // threads per row: four chunks a thread where there are rows to fill the SMs, one where there are few
-    int tpr = 32;
-    const int want = M < 296 ? 1 : 4;
-    while (tpr < kMaxRegThreads && (int64_t)tpr * 8 * want < N) tpr *= 2;
-    int64_t chunks = (N + (int64_t)tpr * 8 - 1) / ((int64_t)tpr * 8);
-    chunks = chunks <= 1 ? 1 : chunks <= 2 ? 2 : chunks <= 4 ? 4 : chunks <= kMaxChunks ? 8 : 0;
-    a.tpr = tpr;
+    // warps per row: `want` spans of 256 columns a warp
+    const int64_t total = (N + 255) / 256;
+    const int want = M < 296 ? 1 : 2;
+    int64_t warps = (total + want - 1) / want;
+    if (warps > kMaxRegThreads / 32) warps = kMaxRegThreads / 32;
+    int64_t spans = (total + warps - 1) / warps;
+    spans = spans <= 4 ? spans : spans <= 8 ? 8 : 0;
+    if (spans > 0 && spans < 8) warps = (total + spans - 1) / spans;
+    a.tpr = (int)warps * 32;
     int rpb = 1;
     if (M >= 296)
-        while (rpb * tpr < 64) rpb *= 2;
+        while (rpb * 2 * a.tpr <= 64) rpb *= 2;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return dtype == DECA_F16 ? launch_out<DECA_F16>(a, out, vec, (int)chunks, rpb, st)
-                             : launch_out<DECA_BF16>(a, out, vec, (int)chunks, rpb, st);
+    return dtype == DECA_F16 ? launch_out<DECA_F16>(a, out, v, (int)spans, rpb, st)
+                             : launch_out<DECA_BF16>(a, out, v, (int)spans, rpb, st);
 }

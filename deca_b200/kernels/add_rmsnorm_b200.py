@@ -2,7 +2,7 @@
 
 from __future__ import annotations
 
-from .module import KernelModule, KernelSpec, _check_view, current_stream_ptr
+from .module import KernelModule, KernelSpec
 
 OUTPUTS = ("same", "e4m3")
 GROUPS = (0, 32, 64, 128, 256)
@@ -31,42 +31,16 @@ def build_add_rmsnorm(mod: KernelSpec) -> KernelModule:
 
 
 def bind(spec: KernelSpec):
-    """Returns main(x, res, w, h, y[, scales]) launching deca_add_rmsnorm on torch's current stream."""
-    import ctypes
-
-    import torch
+    """Returns main(x, res, w[, h, y, scales]) launching deca_add_rmsnorm on torch's current stream; it returns
+    (h, y) or (h, y, scales), made where they are not given."""
+    from functools import partial
 
     from .. import native
 
-    L = native.lib()
     M, N = spec.shape
     out, group = spec.params["out"], spec.params["group"]
     check_add_rmsnorm(M, N, spec.dtype, out, group)
-    code, tdt = native.DTYPE_CODE[spec.dtype], getattr(torch, spec.dtype)
-    eps = ctypes.c_float(spec.params["eps"])
-    eight = out == "e4m3"
-    out_code, out_dt = (native.OUT_E4M3, torch.float8_e4m3fn) if eight else (native.OUT_SAME, tdt)
-    groups = scale_columns(N, group)
-
-    def rows(t, dtype, name, written):
-        _check_view(t, (M, N), dtype, name)
-        if M > 1 and t.stride(0) < N:
-            raise ValueError(f"{name}: rows overlap (row stride {t.stride(0)} for {N} columns)")
-        return t.stride(0)
-
-    def main(x, res, w, h, y, scales=None):
-        sx, sr = rows(x, tdt, "x", False), rows(res, tdt, "res", False)
-        sh, sy = rows(h, tdt, "h", True), rows(y, out_dt, "y", True)
-        _check_view(w, (N,), tdt, "w")
-        if eight:
-            if scales is None:
-                raise ValueError("scales: the e4m3 output needs a tensor for its scales")
-            _check_view(scales, (M, groups), torch.float32, "scales")
-            if not scales.is_contiguous():
-                raise ValueError("scales: expected a contiguous tensor")
-        native.check(
-            L.deca_add_rmsnorm(code, x.data_ptr(), sx, res.data_ptr(), sr, w.data_ptr(), h.data_ptr(), sh, y.data_ptr(), sy,
-                               scales.data_ptr() if eight else None, M, N, eps, out_code, group, current_stream_ptr()),
-            "deca_add_rmsnorm")
-
-    return main
+    launch = native.launch()
+    plan = launch.add_rmsnorm_plan(native.DTYPE_CODE[spec.dtype], M, N, scale_columns(N, group), spec.params["eps"],
+                                   native.OUT_E4M3 if out == "e4m3" else native.OUT_SAME, group)
+    return partial(launch.add_rmsnorm, plan)

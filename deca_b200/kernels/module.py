@@ -67,34 +67,6 @@ def _check_tensor(t, shape, torch_dtype, name):
         raise ValueError(f"{name}: expected a contiguous tensor")
 
 
-def _check_view(t, shape, torch_dtype, name):
-    """A CUDA tensor on the current device whose last dimension is contiguous (other strides are free);
-    ``None`` in ``shape`` stands for any extent."""
-    ok = t.is_cuda and t.dtype == torch_dtype and len(t.shape) == len(shape)
-    if ok:
-        for have, want in zip(t.shape, shape):
-            ok = ok and (want is None or have == want)
-    if not t.is_cuda:
-        raise ValueError(f"{name}: expected a CUDA tensor")
-    if not ok:
-        want = tuple("any" if d is None else d for d in shape)
-        raise ValueError(f"{name}: expected {torch_dtype} of shape {want}, got {t.dtype} of shape {tuple(t.shape)}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name}: the last dimension must be contiguous")
-    _launch_device(t, name)
-
-
-def _launch_device(t, name):
-    """Kernels are launched on the current device's current stream, so tensors must live there; they
-    record no gradient, so a tensor that asks for one is refused."""
-    import torch
-
-    if t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{name}: on cuda:{t.get_device()}, but the current device is cuda:{torch.cuda.current_device()}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name}: requires grad, but this operator records no gradient; call it under torch.no_grad()")
-
-
 @dataclass(frozen=True)
 class BuiltInSchedule:
     """Config of an operator whose kernels choose their own launch shape: there is nothing to tune."""

@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import math
 
-from .module import KernelModule, KernelSpec, _check_view, current_stream_ptr
+from .module import KernelModule, KernelSpec
 
 MAX_REQUESTS = 8192  # the step's prefix sums live in one CTA's shared memory
 PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -47,95 +47,27 @@ def build_paged(mod: KernelSpec) -> KernelModule:
 
 
 def bind_step(spec: KernelSpec):
-    """Returns main(ctx_lens, new_lens, block_table, free_pages, n_free, cu_q, kv_lens, positions, slots,
-    n_free_out, short) launching deca_paged_step on torch's current stream."""
-    import torch
+    """Returns main(ctx_lens, new_lens, block_table, free_pages, n_free[, cu_q, kv_lens, positions, slots, n_free_out,
+    short]) launching deca_paged_step on torch's current stream; it returns the six outputs, made where they
+    are not given."""
+    from functools import partial
 
     from .. import native
 
-    L = native.lib()
-    B, page_size, W, T = spec.shape
-    i32, i64 = torch.int32, torch.int64
-
-    def main(ctx_lens, new_lens, block_table, free_pages, n_free, cu_q, kv_lens, positions, slots, n_free_out, short):
-        _check_view(ctx_lens, (B,), i32, "ctx_lens")
-        _check_view(new_lens, (B,), i32, "new_lens")
-        _check_view(block_table, (B, W), i32, "block_table")
-        _check_view(free_pages, (None,), i32, "free_pages")
-        _check_view(n_free, (1,), i32, "n_free")
-        _check_view(cu_q, (B + 1,), i32, "cu_q")
-        _check_view(kv_lens, (B,), i32, "kv_lens")
-        _check_view(positions, (T,), i32, "positions")
-        _check_view(slots, (T,), i64, "slots")
-        _check_view(n_free_out, (1,), i32, "n_free_out")
-        _check_view(short, (1,), i32, "short")
-        stride = block_table.stride(0) if B > 1 else W
-        if stride < W:
-            raise ValueError(f"block_table: rows overlap (row stride {stride} for {W} entries)")
-        native.check(
-            L.deca_paged_step(ctx_lens.data_ptr(), new_lens.data_ptr(), B, block_table.data_ptr(), stride, W,
-                              free_pages.data_ptr(), free_pages.shape[0], n_free.data_ptr(), page_size, T, cu_q.data_ptr(),
-                              kv_lens.data_ptr(), positions.data_ptr(), slots.data_ptr(), n_free_out.data_ptr(),
-                              short.data_ptr(), current_stream_ptr()), "deca_paged_step")
-
-    return main
+    launch = native.launch()
+    return partial(launch.paged_step, launch.paged_step_plan(*spec.shape))
 
 
 def bind_attn(spec: KernelSpec):
-    """Returns main(q, k_cache, v_cache, block_table, cu_q, kv_lens, out) launching deca_paged_attn on torch's
-    current stream.  The workspace is allocated per call (torch's caching allocator), so calls that
-    overlap, captured ones too, never share one."""
-    import ctypes
-
-    import torch
+    """Returns main(q, k_cache, v_cache, block_table, cu_q, kv_lens[, out]) launching deca_paged_attn on torch's
+    current stream; it returns out.  The workspace is allocated per call."""
+    from functools import partial
 
     from .. import native
 
-    L = native.lib()
     B, H_q, H_kv, D, page_size, max_q, max_kv = spec.shape
     check_attn(B, H_q, H_kv, D, page_size, max_q, max_kv, spec.dtype)
-    tdt, i32 = getattr(torch, spec.dtype), torch.int32
-    a0 = native.PagedAttnArgs(dtype=native.DTYPE_CODE[spec.dtype], B=B, H_q=H_q, H_kv=H_kv, D=D, page_size=page_size,
-                              causal=int(spec.params["causal"]), scale=spec.params["softmax_scale"], max_q=max_q,
-                              max_kv=max_kv)
-    template = bytes(a0)
-    workspace_of = {}  # device -> bytes
-
-    def workspace_bytes(device):
-        n = ctypes.c_size_t()
-        native.check(L.deca_paged_attn_workspace_bytes(ctypes.byref(a0), ctypes.byref(n)), "deca_paged_attn_workspace_bytes")
-        workspace_of[device] = n.value
-        return n.value
-
-    def main(q, k_cache, v_cache, block_table, cu_q, kv_lens, out):
-        _check_view(q, (None, H_q, D), tdt, "q")
-        T = q.shape[0]
-        _check_view(out, (T, H_q, D), tdt, "out")
-        _check_view(k_cache, (None, page_size, H_kv, D), tdt, "k_cache")
-        pages = k_cache.shape[0]
-        _check_view(v_cache, (pages, page_size, H_kv, D), tdt, "v_cache")
-        _check_view(block_table, (B, None), i32, "block_table")
-        _check_view(cu_q, (B + 1,), i32, "cu_q")
-        _check_view(kv_lens, (B,), i32, "kv_lens")
-        if H_q > 1 and out.stride(1) < D or T > 1 and out.stride(0) < 1:
-            raise ValueError(f"out: elements overlap (strides {tuple(out.stride())})")
-        if T == 0:
-            return
-        dev = q.get_device()
-        n = workspace_of.get(dev) or workspace_bytes(dev)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-        a = native.PagedAttnArgs.from_buffer_copy(template)
-        a.T, a.num_pages, a.table_width = T, pages, block_table.shape[1]
-        a.table_stride = block_table.stride(0) if B > 1 else block_table.shape[1]
-        t = a.Q
-        t.data, t.token_stride, t.head_stride = q.data_ptr(), q.stride(0), q.stride(1)
-        t = a.O
-        t.data, t.token_stride, t.head_stride = out.data_ptr(), out.stride(0), out.stride(1)
-        for c, x in ((a.K, k_cache), (a.V, v_cache)):
-            c.data = x.data_ptr()
-            c.page_stride, c.row_stride, c.head_stride, _ = x.stride()
-        a.block_table, a.cu_q, a.kv_lens = block_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr()
-        a.workspace, a.workspace_bytes = ws.data_ptr(), n
-        native.check(L.deca_paged_attn(ctypes.byref(a), current_stream_ptr()), "deca_paged_attn")
-
-    return main
+    launch = native.launch()
+    plan = launch.paged_attn_plan(native.DTYPE_CODE[spec.dtype], B, H_q, H_kv, D, page_size, int(spec.params["causal"]),
+                                  spec.params["softmax_scale"], max_q, max_kv)
+    return partial(launch.paged_attn, plan)

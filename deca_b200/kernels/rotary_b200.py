@@ -18,11 +18,11 @@ from __future__ import annotations
 import math
 from fractions import Fraction
 
-from .module import KernelModule, KernelSpec, _check_view, current_stream_ptr
+from .module import KernelModule, KernelSpec
 
 LAYOUTS = ("half", "interleaved")
 MAX_HEAD_DIM = 256
-PI = Fraction("3.14159265358979323846264338327950288419716939937510")
+PI_BITS = int(Fraction("3.14159265358979323846264338327950288419716939937510") * 2**160)  # pi * 2^160
 
 
 def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None = None):
@@ -59,9 +59,10 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None
 
 
 def fixed_point_turns(freq):
-    """Fractions of a turn per position as 64-bit integers (a turn is 2 ** 64), rounded down.  Rational
+    """Fractions of a turn per position as 64-bit integers (a turn is 2 ** 64), rounded down.  Whole-number
     arithmetic: a double quotient would be off by 4e-7 rad at position 2 ** 31."""
-    return [int(Fraction(f) * 2**63 / PI) % 2**64 for f in freq]
+    ratios = (f.as_integer_ratio() for f in freq)
+    return [(n << 223) // (d * PI_BITS) % 2**64 for n, d in ratios]
 
 
 def check_rotary(D: int, rot_dim: int, layout: str, dtype: str) -> None:
@@ -91,96 +92,32 @@ def build_rotary(mod: KernelSpec) -> KernelModule:
     return KernelModule(mod)
 
 
-def _rotation(D: int, p: dict, inverse: bool):
-    """(native struct, what keeps its host array alive)."""
-    import ctypes
-
+def _plan(launch, dtype: str, D: int, p: dict, H_q: int = 0, H_kv: int = 0, page_size: int = 0):
     from .. import native
 
     freq, amplitude = rotary_frequencies(p["rot_dim"], p["base"], p["scaling"])
-    turns = (ctypes.c_uint64 * len(freq))(*fixed_point_turns(freq))
-    return native.Rotation(D, p["rot_dim"], native.ROT_HALF if p["layout"] == "half" else native.ROT_INTERLEAVED,
-                           int(inverse), amplitude, turns), turns
-
-
-def _tokens(native, t):
-    return native.Tokens(t.data_ptr(), t.stride(0), t.stride(1))
-
-
-def _no_overlap(t, name, size):
-    """A written tensor may not hold an element twice."""
-    if t.shape[0] > 1 and abs(t.stride(0)) < 1 or t.shape[1] > 1 and abs(t.stride(1)) < size:
-        raise ValueError(f"{name}: elements overlap (strides {tuple(t.stride())})")
+    layout = native.ROT_HALF if p["layout"] == "half" else native.ROT_INTERLEAVED
+    return launch.rotary_plan(native.DTYPE_CODE[dtype], D, p["rot_dim"], layout, H_q, H_kv, page_size, amplitude,
+                              fixed_point_turns(freq))
 
 
 def bind(spec: KernelSpec):
-    """Returns main(x, positions, y, inverse=False) launching deca_rotary on torch's current stream."""
-    import ctypes
-
-    import torch
+    """Returns main(x, positions[, y, inverse]) launching deca_rotary on torch's current stream; it returns y."""
+    from functools import partial
 
     from .. import native
 
-    L = native.lib()
-    (D,) = spec.shape
-    code, tdt = native.DTYPE_CODE[spec.dtype], getattr(torch, spec.dtype)
-    forward, keep0 = _rotation(D, spec.params, False)
-    backward, keep1 = _rotation(D, spec.params, True)
-
-    def main(x, positions, y, inverse=False):
-        _check_view(x, (None, None, D), tdt, "x")
-        T, H = x.shape[0], x.shape[1]
-        _check_view(y, (T, H, D), tdt, "y")
-        _check_view(positions, (T,), torch.int32, "positions")
-        _no_overlap(y, "y", D)
-        if T == 0 or H == 0:
-            return
-        xs, ys = _tokens(native, x), _tokens(native, y)
-        native.check(L.deca_rotary(code, ctypes.byref(xs), ctypes.byref(ys), positions.data_ptr(), T, H,
-                                   ctypes.byref(backward if inverse else forward), current_stream_ptr()), "deca_rotary")
-
-    main._keepalive = (keep0, keep1)
-    return main
+    launch = native.launch()
+    return partial(launch.rotary, _plan(launch, spec.dtype, *spec.shape, spec.params))
 
 
 def bind_append(spec: KernelSpec):
-    """Returns main(q, k, v, positions, slots, k_cache, v_cache, q_out) launching deca_rotary_append on
-    torch's current stream."""
-    import ctypes
-
-    import torch
+    """Returns main(q, k, v, positions, slots, k_cache, v_cache[, q_out]) launching deca_rotary_append on torch's
+    current stream; it returns q_out."""
+    from functools import partial
 
     from .. import native
 
-    L = native.lib()
+    launch = native.launch()
     H_q, H_kv, D, page_size = spec.shape
-    code, tdt = native.DTYPE_CODE[spec.dtype], getattr(torch, spec.dtype)
-    rotation, keep = _rotation(D, spec.params, False)
-    rot = ctypes.byref(rotation)
-
-    def cache(t):
-        return native.Cache(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
-
-    def main(q, k, v, positions, slots, k_cache, v_cache, q_out):
-        _check_view(q, (None, H_q, D), tdt, "q")
-        T = q.shape[0]
-        _check_view(k, (T, H_kv, D), tdt, "k")
-        _check_view(v, (T, H_kv, D), tdt, "v")
-        _check_view(q_out, (T, H_q, D), tdt, "q_out")
-        _check_view(positions, (T,), torch.int32, "positions")
-        _check_view(slots, (T,), torch.int64, "slots")
-        _check_view(k_cache, (None, page_size, H_kv, D), tdt, "k_cache")
-        pages = k_cache.shape[0]
-        _check_view(v_cache, (pages, page_size, H_kv, D), tdt, "v_cache")
-        _no_overlap(q_out, "q_out", D)
-        if T == 0:
-            return
-        qs, ks, vs, qo, kc, vc = (_tokens(native, q), _tokens(native, k), _tokens(native, v), _tokens(native, q_out),
-                                  cache(k_cache), cache(v_cache))
-        r = ctypes.byref
-        native.check(L.deca_rotary_append(code, r(qs), r(ks), r(vs), r(qo), r(kc), r(vc), positions.data_ptr(),
-                                          slots.data_ptr(), T, H_q, H_kv, pages, page_size, rot, current_stream_ptr()),
-                     "deca_rotary_append")
-
-    main._keepalive = keep
-    return main
+    return partial(launch.rotary_append, _plan(launch, spec.dtype, D, spec.params, H_q, H_kv, page_size))

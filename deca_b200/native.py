@@ -120,6 +120,19 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+def launch():
+    """The extension that checks and launches the serving operators; raises if it has not been built."""
+    lib()
+    try:
+        from . import _launch
+    except ImportError as e:
+        raise RuntimeError(
+            f"deca_b200/_launch.so cannot be loaded ({e}): the serving operators are not built and there is no "
+            "fallback. Run `python -m deca_b200.build`."
+        ) from e
+    return _launch
+
+
 def version() -> str:
     return lib().deca_version().decode()
 

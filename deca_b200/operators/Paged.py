@@ -43,28 +43,16 @@ class PagedStep(Operator):
 
         return build_paged(mod)
 
-    def make_output(self, device="cuda"):
-        import torch
-
-        i32 = {"dtype": torch.int32, "device": device}
-        return PagedStepResult(torch.empty(self.B + 1, **i32), torch.empty(self.B, **i32), torch.empty(self.max_tokens, **i32),
-                               torch.empty(self.max_tokens, dtype=torch.int64, device=device), torch.empty(1, **i32),
-                               torch.empty(1, **i32))
-
     def __call__(self, ctx_lens, new_lens, block_table, free_pages, n_free, out: PagedStepResult | None = None):
         """ctx_lens, new_lens [B], block_table [B, table_width], free_pages [F], n_free [1], all int32.
 
         Pages for the new tokens are taken from the end of ``free_pages[:n_free]`` in request order and written
         to ``block_table`` in place (-1 where the list has run out).  Returns cu_q [B + 1], kv_lens [B],
-        positions and slots [max_tokens], n_free [1] and short [1] (pages that were missing; 0: none) in
-        tensors that may not be the inputs' own."""
+        positions and slots [max_tokens], n_free [1] and short [1] (pages that were missing; 0: none), in the
+        tensors of ``out`` (the result of another call, say), which may not be the inputs' own."""
         if self._mod is None:
             self._mod = self.compile(self.build_mod())["main"]
-        if out is None:
-            out = self.make_output(ctx_lens.device)
-        self._mod(ctx_lens, new_lens, block_table, free_pages, n_free, out.cu_q, out.kv_lens, out.positions, out.slots,
-                  out.n_free, out.short)
-        return out
+        return PagedStepResult(*self._mod(ctx_lens, new_lens, block_table, free_pages, n_free, *(out or ())))
 
     def describe(self) -> str:
         return (f"{self.name}(B={self.B}, page_size={self.page_size}, table_width={self.table_width}, "
@@ -127,14 +115,9 @@ class PagedAttention(Operator):
         """q [T, H_q, D]: request r owns rows cu_q[r] .. cu_q[r + 1] - 1; caches [pages, page_size, H_kv, D];
         block_table [B, width], cu_q [B + 1], kv_lens [B], int32 on the device.  Returns O [T, H_q, D].  Rows that
         belong to no request are not written."""
-        import torch
-
         if self._mod is None:
             self._mod = self.compile(self.build_mod())["main"]
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        self._mod(q, k_cache, v_cache, block_table, cu_q, kv_lens, out)
-        return out
+        return self._mod(q, k_cache, v_cache, block_table, cu_q, kv_lens, out)
 
     def make_inputs(self):
         """A full batch from one seeded generator: max_q new tokens behind max_kv - max_q, pages in random order."""

@@ -49,14 +49,9 @@ class Rotary(Operator):
 
     def __call__(self, x, positions, out=None, inverse: bool = False):
         """Returns x [T, H, D] turned by ``positions`` [T] (int32); ``out`` may be ``x``."""
-        import torch
-
         if self._mod is None:
             self._mod = self.compile(self.build_mod())["main"]
-        if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        self._mod(x, positions, out, inverse)
-        return out
+        return self._mod(x, positions, out, inverse)
 
     def describe(self) -> str:
         return f"{self.name}(D={self.D}, rot_dim={self.rot_dim}, {self.layout}, {self.dtype})"
@@ -84,14 +79,9 @@ class RotaryAppend(Rotary):
     def __call__(self, q, k, v, positions, slots, k_cache, v_cache, out=None):
         """q [T, H_q, D], k and v [T, H_kv, D] (views of one projection will do), positions [T] int32, slots [T]
         int64; returns the turned q (``out`` may be ``q``)."""
-        import torch
-
         if self._mod is None:
             self._mod = self.compile(self.build_mod())["main"]
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        self._mod(q, k, v, positions, slots, k_cache, v_cache, out)
-        return out
+        return self._mod(q, k, v, positions, slots, k_cache, v_cache, out)
 
     def describe(self) -> str:
         return (f"{self.name}(H_q={self.H_q}, H_kv={self.H_kv}, D={self.D}, page_size={self.page_size}, "

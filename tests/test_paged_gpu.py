@@ -84,7 +84,7 @@ def test_step_refusals():
     for bad in [(a.long(), b, table, free, n), (a, b[:1], table, free, n), (a, b, table[:, :3], free, n), (a, b, table, free, n[0])]:
         with pytest.raises(ValueError):
             op(*bad)
-    out = op.make_output()
+    out = op(a, b, table, free, n)
     with pytest.raises(RuntimeError):
         op(a, b, table, free, n, out=out._replace(kv_lens=a))
     for bad in ((0, 16, 4, 8), (8193, 16, 4, 8), (2, 24, 4, 8), (2, 16, 2**28, 8)):

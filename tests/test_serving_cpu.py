@@ -124,3 +124,28 @@ def test_attention_entry_refuses(native):
                      ({"Q": native.Tokens(p + 8, 256, 64)}, -3), ({"Q": native.Tokens(p, 252, 64)}, -3), ({"K": native.Cache(p, 2048, 130, 64)}, -3),
                      ({"block_table": p + 2}, -3)):
         assert L.deca_paged_attn_check(args(**kw)) == code, kw
+
+
+def test_calls_refuse_what_is_not_on_a_gpu():
+    import torch
+
+    from deca_b200.operators import AddRMSNorm, PagedAttention, PagedStep, Rotary, RotaryAppend
+
+    x, i = torch.ones(4, 64, dtype=torch.float16), torch.ones(4, dtype=torch.int32)
+    for op, args in ((AddRMSNorm(4, 64), (x, x, x[0])), (Rotary(64), (x[:, None], i)), (RotaryAppend(1, 1, 64, 16), (x[:, None],) * 3 + (i,) * 2 + (x,) * 2),
+                     (PagedStep(4, 16, 2, 4), (i,) * 5), (PagedAttention(4, 1, 1, 64, 16, 1, 1), (x[:, None],) * 3 + (i,) * 3)):
+        with pytest.raises(ValueError, match="CUDA"):
+            op(*args)
+        with pytest.raises(TypeError):
+            op(3, *args[1:])
+
+
+def test_missing_extension_fails_loudly(native, monkeypatch):
+    import sys
+
+    from deca_b200.operators import AddRMSNorm
+
+    monkeypatch.setitem(sys.modules, "deca_b200._launch", None)
+    monkeypatch.delattr("deca_b200._launch", raising=False)
+    with pytest.raises(RuntimeError, match="no fallback"):
+        AddRMSNorm(4, 64)(None, None, None)
