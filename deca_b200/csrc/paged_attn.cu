@@ -1,9 +1,12 @@
 // Entry points of the paged attention: argument rules, choice of the schedule, workspace.
+#include <cmath>
+
 #include "paged_attn.cuh"
 
 namespace deca {
+int paged_rows_ctas(int D, int mt, int sms);
 size_t paged_rows_workspace(int D, int mt, int sms);
-int paged_rows_launch(int dtype, PagedArgs &g, int D, int mt, int sms, void *workspace, cudaStream_t st);
+int paged_rows_launch(const deca_paged_attn_args &a, PagedArgs &g, int mt, bool cut, int sms, cudaStream_t st);
 size_t paged_tiles_workspace(int D, int sms);
 int paged_tiles_launch(const deca_paged_attn_args &a, PagedArgs &g, int sms, cudaStream_t st);
 
@@ -22,6 +25,18 @@ int row_tiles(const deca_paged_attn_args &a) { return (int64_t)a.max_q * (a.H_q 
 // The tensor-core tiles take what has more than 32 query rows per request and key head.
 bool use_tiles(const deca_paged_attn_args &a) {
     return (int64_t)a.max_q * (a.H_q / a.H_kv) > 32 && a.scale > 0.f;  // the tiles keep maxima of unscaled scores
+}
+// Whether the streaming schedule cuts items.  Whole, a (request, key head) pair is one CTA's and costs nothing but
+// its keys; cut, the CTAs share the keys evenly, which costs 10 - 15 us of partial results and joining.  Measured
+// (D = 128, 8 key heads, whole / cut): 16 x 2000 keys 28.7 / 31.5 us, 32 x 500 .. 2500 43 / 48, 256 x 100 .. 500
+// 67 / 87; but 4 x 4000 49 / 21, 1 x 8192 93 / 18, 64 x 1000 .. 8191 226 / 214.
+bool use_cuts(const deca_paged_attn_args &a, int sms) {
+    if (a.max_kv <= 768) return false;
+    const double pairs = (double)a.B * a.H_kv, ctas = paged_rows_ctas(a.D, row_tiles(a), sms);
+    if (8 * pairs < 3 * ctas) return true;
+    // microseconds of reading half of the longest contexts, and the share of them that the last round idles
+    const double us = pairs * a.max_kv * a.D * 2.0 / 6.5e6, rounds = std::ceil(pairs / ctas);
+    return pairs <= ctas ? us > 60 : us * (rounds * ctas / pairs - 1.0) > 15;
 }
 // ... and tensor maps want strides that advance
 bool strides_ok(const PagedArgs &g) {
@@ -56,7 +71,7 @@ extern "C" int deca_paged_attn_workspace_bytes(const deca_paged_attn_args *a, si
     if ((a->D != 64 && a->D != 128) || a->H_kv < 1) return DECA_ERR_UNSUPPORTED;
     DeviceInfo di;
     if (int rc = current_device_info(&di)) return rc;
-    *bytes = paged_rows_workspace(a->D, row_tiles(*a), di.sms);
+    *bytes = use_cuts(*a, di.sms) ? paged_rows_workspace(a->D, row_tiles(*a), di.sms) : 0;
     if (use_tiles(*a) && paged_tiles_workspace(a->D, di.sms) > *bytes) *bytes = paged_tiles_workspace(a->D, di.sms);
     return DECA_OK;
 }
@@ -66,7 +81,7 @@ extern "C" int deca_paged_attn(const deca_paged_attn_args *a, void *stream) {
     if (a->T == 0) return DECA_OK;
     size_t need = 0;
     if (int rc = deca_paged_attn_workspace_bytes(a, &need)) return rc;
-    if (!a->workspace) return DECA_ERR_NULL;
+    if (need > 0 && !a->workspace) return DECA_ERR_NULL;
     if (!aligned_to(a->workspace, 256)) return DECA_ERR_ALIGN;
     if (a->workspace_bytes < need) return DECA_ERR_SCRATCH_LIMIT;
     DeviceInfo di;
@@ -86,8 +101,8 @@ extern "C" int deca_paged_attn(const deca_paged_attn_args *a, void *stream) {
     if (!g.status) return (int)cudaErrorUnknown;
     if (use_tiles(*a) && strides_ok(g)) {
         g.min_steps = 2;
+        g.max_parts = 1 << 20;
         return paged_tiles_launch(*a, g, di.sms, static_cast<cudaStream_t>(stream));
     }
-    g.min_steps = 4;
-    return paged_rows_launch(a->dtype, g, a->D, row_tiles(*a), di.sms, a->workspace, static_cast<cudaStream_t>(stream));
+    return paged_rows_launch(*a, g, row_tiles(*a), use_cuts(*a, di.sms), di.sms, static_cast<cudaStream_t>(stream));
 }

@@ -23,19 +23,24 @@ struct PagedArgs {
     long long table_stride;
     long long T, num_pages;
     int B, W, Hkv, group;  // group: query heads per key head
+    int tile_tokens;       // TokenTiles: whole tokens in 128 rows
     int page_shift;
     int causal;
     float sl2;  // scale * log2 e
-    int whole;  // 1: items are not cut (no partial results)
     int min_steps;  // fewest steps worth a CTA of their own
+    int max_parts;  // most CTAs per request and key head, on average
     float *part;    // partial results, 2 per CTA
-    struct PartialItem *meta;  // one per CTA
+    struct PartialItem *meta;     // one per CTA (tiles)
+    unsigned long long *flags;    // 2 per CTA (rows): `tag` where the partial result is complete
+    unsigned long long tag;       // this launch's
     DeviceStatus *status;
 };
 
 // The item that starts in a CTA's range and ends in a later one's; `last` < 0: none.
 struct PartialItem {
-    int req, head, tile, last;
+    int last;        // the CTA that ends it
+    int head, tile;
+    int q0, n;       // of its request
 };
 
 struct ReqView {
@@ -66,19 +71,24 @@ template <int ROWS_, int KEYS>
 struct PackedRows {
     static constexpr int ROWS = ROWS_;
     // token of the request and head of the group in `row` of a tile; false: the row is not in use
-    static __device__ __forceinline__ bool place(const PagedArgs &g, const ReqView &v, int tile, int row, int &tok, int &j) {
-        const long long packed = (long long)tile * ROWS + row;
-        tok = (int)min(packed / g.group, (long long)v.n);
-        j = (int)(packed % g.group);
-        return tok < v.n;
+    static __device__ __forceinline__ bool place(const PagedArgs &g, int n, int tile, int row, int &tok, int &j) {
+        const unsigned long long packed = (unsigned long long)tile * ROWS + row;
+        const unsigned long long t = packed / (unsigned)g.group;
+        tok = (int)min(t, (unsigned long long)n);
+        j = (int)(packed - t * (unsigned)g.group);
+        return tok < n;
     }
     static __device__ __forceinline__ int tiles(const PagedArgs &g, const ReqView &v) {
-        return (int)(((long long)v.n * g.group + ROWS - 1) / ROWS);
+        return (int)(((unsigned long long)v.n * (unsigned)g.group + ROWS - 1) / ROWS);
+    }
+    // the last token of a tile; the division only where more tiles follow
+    static __device__ __forceinline__ int last_token(const PagedArgs &g, const ReqView &v, int tile) {
+        const unsigned long long end = (unsigned long long)(tile + 1) * ROWS;
+        if (end >= (unsigned long long)v.n * (unsigned)g.group) return v.n - 1;
+        return (int)((end - 1) / (unsigned)g.group);
     }
     static __device__ __forceinline__ int steps(const PagedArgs &g, const ReqView &v, int tile) {
-        const long long last_row = min((long long)(tile + 1) * ROWS, (long long)v.n * g.group) - 1;
-        const int keys = keys_until(v, (int)(last_row / g.group));
-        return max((keys + KEYS - 1) / KEYS, 1);
+        return max((keys_until(v, last_token(g, v, tile)) + KEYS - 1) / KEYS, 1);
     }
     static __device__ __forceinline__ long long head_steps(const PagedArgs &g, const ReqView &v) {
         long long s = 0;
@@ -92,12 +102,12 @@ struct PackedRows {
 template <int KEYS>
 struct TokenTiles {
     static constexpr int ROWS = 256;
-    static __device__ __forceinline__ int tokens(const PagedArgs &g) { return 128 / g.group; }  // of one of the two
-    static __device__ __forceinline__ bool place(const PagedArgs &g, const ReqView &v, int tile, int row, int &tok, int &j) {
-        const int r = row & 127, t = r / g.group, n = tokens(g);
-        tok = (2 * tile + (row >> 7)) * n + t;
+    static __device__ __forceinline__ int tokens(const PagedArgs &g) { return g.tile_tokens; }  // of one of the two
+    static __device__ __forceinline__ bool place(const PagedArgs &g, int n, int tile, int row, int &tok, int &j) {
+        const int r = row & 127, t = r / g.group;
+        tok = (2 * tile + (row >> 7)) * tokens(g) + t;
         j = r - t * g.group;
-        return t < n && tok < v.n;
+        return t < tokens(g) && tok < n;
     }
     static __device__ __forceinline__ int tiles(const PagedArgs &g, const ReqView &v) {
         const int n = 2 * tokens(g);
@@ -118,82 +128,135 @@ struct TokenTiles {
 // A CTA's place in the list of items.
 struct WorkPos {
     int req, head, tile;
-    int step;          // first step of the current item that is this CTA's
-    long long left;    // steps this CTA still has to take
-    long long base;    // global number of the current item's first step
-    long long total;   // U
-    int ctas;          // CTAs that share the work
+    int step;  // first step of the current item that is this CTA's
+    int left;  // steps this CTA still has to take
+};
+// The CTA's range in the list; kept in shared memory, read where an item is cut.
+struct WorkShare {
+    long long begin, end, total;  // its first step, one past its last; steps in all
+    int ctas;              // CTAs that share the work
+    WorkPos first;
+    long long warp_sum[32];
 };
 
-// Finds the CTA's first item.  Called by all threads of the CTA (block barriers inside); `scratch` holds
-// 34 long longs plus one WorkPos in shared memory.
+// Finds the CTA's first item.  Called by all threads of the CTA (block barriers inside); `costs` is shared
+// memory for `room` requests' costs, free afterwards.
 template <typename TL>
-__device__ __forceinline__ bool find_work(const PagedArgs &g, WorkPos &out, long long *scratch) {
+__device__ __forceinline__ bool find_work(const PagedArgs &g, WorkPos &out, WorkShare *share, unsigned long long *costs, int room) {
     const int nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = nt >> 5;
-    WorkPos *found = reinterpret_cast<WorkPos *>(scratch + 34);
+    auto cost_of = [&](int r) { return (unsigned long long)(TL::head_steps(g, request_view(g, r)) * g.Hkv); };
+    // side by side through the requests' lengths, then each thread sums the costs of neighbours
+    for (int r = tid; r < min(g.B, room); r += nt) costs[r] = cost_of(r);
+    if (tid == 0) share->first.req = -1;
+    __syncthreads();
     const int per = (g.B + nt - 1) / nt;
     const int r0 = min(tid * per, g.B), r1 = min(r0 + per, g.B);
-    long long mine = 0;
-    for (int r = r0; r < r1; ++r) mine += TL::head_steps(g, request_view(g, r)) * g.Hkv;
-    long long inc = mine;
+    auto cost_at = [&](int r) { return r < room ? costs[r] : cost_of(r); };
+    unsigned long long mine = 0;
+    for (int r = r0; r < r1; ++r) mine += cost_at(r);
+    unsigned long long inc = mine;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
-        const long long a = __shfl_up_sync(0xFFFFFFFFu, inc, s);
+        const unsigned long long a = __shfl_up_sync(0xFFFFFFFFu, inc, s);
         if (lane >= s) inc += a;
     }
-    if (lane == 31) scratch[warp] = inc;
-    if (tid == 0) found->req = -1;
+    if (lane == 31) share->warp_sum[warp] = (long long)inc;
     __syncthreads();
-    long long before = 0, total = 0;
+    unsigned long long before = 0, total = 0;
     for (int w = 0; w < nw; ++w) {
-        if (w < warp) before += scratch[w];
-        total += scratch[w];
+        if (w < warp) before += share->warp_sum[w];
+        total += share->warp_sum[w];
     }
     before += inc - mine;
-    int ctas = (int)gridDim.x;
-    const long long most = (total + g.min_steps - 1) / g.min_steps;
-    if (most < ctas) ctas = (int)most;
-    const int c = (int)blockIdx.x;
+    const unsigned long long most = min((total + g.min_steps - 1) / (unsigned)g.min_steps,
+                                        (unsigned long long)g.B * (unsigned)g.Hkv * (unsigned)g.max_parts);
+    const unsigned ctas = most < gridDim.x ? (unsigned)most : gridDim.x, c = blockIdx.x;
     if (c < ctas) {
-        const long long u0 = total * c / ctas, u1 = total * (c + 1) / ctas;
+        const unsigned long long u0 = total * c / ctas;
         if (u0 >= before && u0 < before + mine) {  // one thread: the one whose requests hold step u0
-            long long at = before;
-            for (int r = r0; r < r1; ++r) {
-                const ReqView v = request_view(g, r);
-                const long long per_head = TL::head_steps(g, v);
-                const long long all = per_head * g.Hkv;
-                if (u0 >= at + all) {
-                    at += all;
-                    continue;
-                }
-                const int head = (int)((u0 - at) / per_head);
-                at += per_head * head;
-                int tile = 0;
-                while (true) {
-                    const int s = TL::steps(g, v, tile);
-                    if (u0 < at + s) break;
-                    at += s;
-                    ++tile;
-                }
-                found->req = r, found->head = head, found->tile = tile;
-                found->step = (int)(u0 - at);
-                found->left = u1 - u0;
-                found->base = at;
-                found->total = total;
-                found->ctas = ctas;
-                break;
-            }
+            unsigned long long at = before;
+            int r = r0;
+            for (; u0 >= at + cost_at(r); ++r) at += cost_at(r);
+            const ReqView v = request_view(g, r);
+            const unsigned long long per_head = cost_at(r) / (unsigned)g.Hkv;
+            const int head = (int)((u0 - at) / per_head);
+            at += per_head * head;
+            int tile = 0;
+            for (int s; u0 >= at + (s = TL::steps(g, v, tile)); ++tile) at += s;
+            const unsigned long long u1 = total * (c + 1) / ctas;
+            share->first.req = r, share->first.head = head, share->first.tile = tile;
+            share->first.step = (int)(u0 - at);
+            share->first.left = (int)min(u1 - u0, 2147483647ull);
+            share->begin = (long long)u0;
+            share->end = (long long)u1;
+            share->total = (long long)total;
+            share->ctas = (int)ctas;
         }
     }
     __syncthreads();
-    out = *found;
+    out = share->first;
     return out.req >= 0;
+}
+
+// Few items (at most half as many as CTAs, of at most 32 requests): instead of an equal run of steps each CTA gets
+// one part of one item, so that none pays the start and end of two.  Items are cut into parts of at most C
+// steps, C = steps / (CTAs - items) rounded up, which needs no more parts than CTAs.  Every warp finds its CTA's part
+// by itself (lane r holds request r).  Returns 0 where there are too many items, 1 with a part, -1 without.
+template <typename TL>
+__device__ __forceinline__ int find_part(const PagedArgs &g, WorkPos &w, ReqView &v, int &part, int &parts) {
+    if (g.B > 32) return 0;
+    const int lane = threadIdx.x & 31;
+    ReqView mine = {0, 0, 0, 0};
+    int tiles = 0;
+    unsigned long long steps = 0;
+    if (lane < g.B) {
+        mine = request_view(g, lane);
+        tiles = TL::tiles(g, mine);
+        if (2ll * tiles * g.Hkv > (int)gridDim.x) tiles = (int)gridDim.x;  // too many: said below
+        for (int t = 0; t < tiles; ++t) steps += TL::steps(g, mine, t);
+    }
+    unsigned long long total = steps;
+    int items = tiles;
+#pragma unroll
+    for (int s = 16; s >= 1; s >>= 1) {
+        total += __shfl_xor_sync(0xFFFFFFFFu, total, s);
+        items += __shfl_xor_sync(0xFFFFFFFFu, items, s);
+    }
+    total *= (unsigned)g.Hkv;
+    if (2ll * items * g.Hkv > (int)gridDim.x) return 0;
+    if (items == 0) return -1;
+    items *= g.Hkv;
+    const unsigned room = gridDim.x - (unsigned)items;
+    const int most = (int)max((total + room - 1) / room, (unsigned long long)g.min_steps);
+    auto parts_of = [&](const ReqView &q, int t) { return (TL::steps(g, q, t) + most - 1) / most; };
+    int count = 0;  // parts of one key head of this lane's request
+    for (int t = 0; t < tiles; ++t) count += parts_of(mine, t);
+    int end = count * g.Hkv;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+        const int a = __shfl_up_sync(0xFFFFFFFFu, end, s);
+        if (lane >= s) end += a;
+    }
+    const int at = (int)blockIdx.x - (end - count * g.Hkv);  // the CTA's place among this lane's parts
+    const unsigned owner = __ballot_sync(0xFFFFFFFFu, at >= 0 && at < count * g.Hkv);
+    if (owner == 0) return -1;
+    const int r = __ffs((int)owner) - 1;
+    v.q0 = __shfl_sync(0xFFFFFFFFu, mine.q0, r), v.n = __shfl_sync(0xFFFFFFFFu, mine.n, r);
+    v.kv = __shfl_sync(0xFFFFFFFFu, mine.kv, r), v.shift = __shfl_sync(0xFFFFFFFFu, mine.shift, r);
+    const int per_head = __shfl_sync(0xFFFFFFFFu, count, r);
+    part = __shfl_sync(0xFFFFFFFFu, at, r);
+    w.req = r, w.head = part / per_head, w.tile = 0;
+    part -= w.head * per_head;
+    for (; part >= (parts = parts_of(v, w.tile)); ++w.tile) part -= parts;
+    const unsigned long long all = (unsigned)TL::steps(g, v, w.tile);
+    w.step = (int)(all * (unsigned)part / (unsigned)parts);
+    w.left = (int)(all * (unsigned)(part + 1) / (unsigned)parts) - w.step;
+    return 1;
 }
 
 // Moves on to the next item of the list; false behind the last one.
 template <typename TL>
 __device__ __forceinline__ bool next_item(const PagedArgs &g, WorkPos &w, ReqView &v) {
-    w.base += TL::steps(g, v, w.tile);
     w.step = 0;
     if (++w.tile < TL::tiles(g, v)) return true;
     w.tile = 0;
@@ -206,76 +269,116 @@ __device__ __forceinline__ bool next_item(const PagedArgs &g, WorkPos &w, ReqVie
     return false;
 }
 
-// The CTA that takes global step x.
-__device__ __forceinline__ int cta_of_step(const WorkPos &w, long long x) {
-    return (int)(((x + 1) * w.ctas - 1) / w.total);
+// The CTA that takes step x: the last c with total * c / ctas <= x.
+__device__ __forceinline__ int cta_of(const WorkShare *share, long long x) {
+    return (int)(((unsigned long long)(x + 1) * (unsigned)share->ctas - 1) / (unsigned long long)share->total);
 }
 
 // Floats of one partial result: ROWS x D numerators, then ROWS maxima and ROWS sums.
 template <int ROWS, int D>
 constexpr size_t kPartFloats = (size_t)ROWS * D + 2 * ROWS;
 
-// Joins the partial results of cut items (kernel launched behind either schedule).
-template <int DT, int D, typename TL>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs g) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const PartialItem it = g.meta[blockIdx.x];
-    if (it.last < 0) return;
-    const ReqView v = request_view(g, it.req);
-    const int lane = threadIdx.x & 31;
-    constexpr int ROWS = TL::ROWS;
-    const int row = blockIdx.y * 4 + (threadIdx.x >> 5);
-    int tok, j;
-    if (!TL::place(g, v, it.tile, row, tok, j)) return;
-    const int c0 = (int)blockIdx.x, n = it.last - c0 + 1;
-    // part i: the CTA that starts the item keeps it in its second slot, the following ones in their first
-    auto part = [&](int i) { return g.part + ((size_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats<ROWS, D>; };
-    float top = -INFINITY;
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, part(i)[(size_t)ROWS * D + row]);
-#pragma unroll
-    for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
-    const float base = top == -INFINITY ? 0.f : top;
+// One row of a cut item from its n parts, by one warp.  Lane i reads the statistics of part i (of 32) while the
+// numerators of BATCH parts are on their way.  part(i): the i-th part; acc: D / 32 columns of this lane.
+template <int ROWS, int D, int BATCH, typename Part>
+__device__ __forceinline__ void join_row(Part part, int n, int row, int lane, float (&acc)[D / 32], float &sum) {
     constexpr int PER = D / 32;
-    float acc[PER] = {}, sum = 0.f;
+    float top = -INFINITY;
+    sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) acc[k] = 0.f;
+#pragma unroll 1
     for (int i0 = 0; i0 < n; i0 += 32) {
-        float wt = 0.f, l = 0.f;
+        float m = -INFINITY, l = 0.f;
         if (i0 + lane < n) {
-            const float *p = part(i0 + lane);
-            wt = exp2f(p[(size_t)ROWS * D + row] - base);
-            l = p[(size_t)ROWS * D + ROWS + row];
+            const float *p = part(i0 + lane) + (size_t)ROWS * D + row;
+            m = __ldcg(p), l = __ldcg(p + ROWS);
         }
-        const int m = min(32, n - i0);
-#pragma unroll 4
-        for (int i = 0; i < m; ++i) {
-            const float w = __shfl_sync(0xFFFFFFFFu, wt, i);
-            sum = fmaf(w, __shfl_sync(0xFFFFFFFFu, l, i), sum);
-            const float *p = part(i0 + i) + (size_t)row * D + lane * PER;
-            if constexpr (PER == 4) {
-                const float4 x = *reinterpret_cast<const float4 *>(p);
-                acc[0] = fmaf(w, x.x, acc[0]), acc[1] = fmaf(w, x.y, acc[1]);
-                acc[2] = fmaf(w, x.z, acc[2]), acc[3] = fmaf(w, x.w, acc[3]);
-            } else {
-                const float2 x = *reinterpret_cast<const float2 *>(p);
-                acc[0] = fmaf(w, x.x, acc[0]), acc[1] = fmaf(w, x.y, acc[1]);
+        float wt = 0.f;
+#pragma unroll 1
+        for (int b0 = 0; b0 < 32 && i0 + b0 < n; b0 += BATCH) {
+            float x[BATCH][PER];
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+#pragma unroll
+                for (int k = 0; k < PER; ++k) x[b][k] = 0.f;
+                if (i0 + b0 + b < n) {
+                    const float *p = part(i0 + b0 + b) + (size_t)row * D;
+                    if constexpr (PER == 4) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(p) + lane);
+                        x[b][0] = v.x, x[b][1] = v.y, x[b][2] = v.z, x[b][3] = v.w;
+                    } else {
+                        const float2 v = __ldcg(reinterpret_cast<const float2 *>(p) + lane);
+                        x[b][0] = v.x, x[b][1] = v.y;
+                    }
+                }
+            }
+            if (b0 == 0) {  // weights of these 32 parts, and what came before brought to the same maximum
+                float up = m;
+#pragma unroll
+                for (int s = 16; s >= 1; s >>= 1) up = fmaxf(up, __shfl_xor_sync(0xFFFFFFFFu, up, s));
+                up = fmaxf(up, top);
+                const float base = up == -INFINITY ? 0.f : up;
+                wt = exp2f(m - base);
+                const float old = exp2f(top - base);
+                top = up;
+                float part_sum = wt * l;
+#pragma unroll
+                for (int s = 16; s >= 1; s >>= 1) part_sum += __shfl_xor_sync(0xFFFFFFFFu, part_sum, s);
+                sum = fmaf(sum, old, part_sum);
+#pragma unroll
+                for (int k = 0; k < PER; ++k) acc[k] *= old;
+            }
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                const float w = __shfl_sync(0xFFFFFFFFu, wt, (b0 + b) & 31);
+                if (i0 + b0 + b >= n) continue;
+#pragma unroll
+                for (int k = 0; k < PER; ++k) acc[k] = fmaf(w, x[b][k], acc[k]);
             }
         }
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    const int head = it.head * g.group + j;
-    char *o = g.o + 2 * (((long long)v.q0 + tok) * g.o_st + head * g.o_sh + lane * PER);
-    if constexpr (PER == 4)
-        *reinterpret_cast<uint2 *>(o) = make_uint2(Pack16<DT>::pack(acc[0] * inv, acc[1] * inv), Pack16<DT>::pack(acc[2] * inv, acc[3] * inv));
-    else
-        *reinterpret_cast<uint32_t *>(o) = Pack16<DT>::pack(acc[0] * inv, acc[1] * inv);
 }
+
+template <int DT, int D>
+__device__ __forceinline__ void store_joined(char *row, int lane, const float (&acc)[D / 32], float sum) {
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    if constexpr (D == 128)
+        *reinterpret_cast<uint2 *>(row + lane * 8) =
+            make_uint2(Pack16<DT>::pack(acc[0] * inv, acc[1] * inv), Pack16<DT>::pack(acc[2] * inv, acc[3] * inv));
+    else
+        *reinterpret_cast<uint32_t *>(row + lane * 4) = Pack16<DT>::pack(acc[0] * inv, acc[1] * inv);
+}
+
+// Joins the items that the tiles' CTAs have cut: a kernel behind theirs.
+constexpr int kJoinThreads = 256;
+template <int DT, int D, typename TL>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs g) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const PartialItem it = g.meta[blockIdx.x];
+    if (it.last < 0) return;
+    const int lane = threadIdx.x & 31, c0 = (int)blockIdx.x;
+    // part i: the CTA that starts the item keeps it in its second slot, the following ones in their first
+    auto part = [&](int i) { return g.part + ((size_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats<TL::ROWS, D>; };
+    for (int row = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); row < TL::ROWS; row += gridDim.y * (kJoinThreads / 32)) {
+        int tok, j;
+        if (!TL::place(g, it.n, it.tile, row, tok, j)) continue;
+        float acc[D / 32], sum;
+        join_row<TL::ROWS, D, 4>(part, it.last - c0 + 1, row, lane, acc, sum);
+        store_joined<DT, D>(g.o + 2 * (((long long)it.q0 + tok) * g.o_st + (long long)(it.head * g.group + j) * g.o_sh), lane, acc, sum);
+    }
+}
+
+// Lets the next kernel of the stream be scheduled while this one drains (it waits for the results itself).
+__device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // Launches the join behind the kernel last launched on the stream; its blocks may be scheduled while
 // that kernel drains and wait for its results on the device.
 template <int DT, int D, typename TL>
-int launch_join(const PagedArgs &g, unsigned ctas, cudaStream_t st) {
+int launch_join(const PagedArgs &g, unsigned ctas, unsigned blocks, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas, TL::ROWS / 4);
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3(ctas, blocks);
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -11,13 +11,13 @@
 //
 // The running maximum moves only when a score exceeds it by 2^8 (it then rescales the numerators);
 // otherwise the exponentials are taken against the old one, as in the dense attention kernels.
+#include <atomic>
+#include <random>
+
 #include "paged_attn.cuh"
 
 namespace deca {
 namespace {
-
-constexpr int kThreads = 128;
-constexpr int kKeys = 64;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
@@ -57,47 +57,56 @@ __device__ __forceinline__ bool pair_not_finite(uint32_t w) {
     return (w & e) == e || ((w >> 16) & e) == e;
 }
 
-template <int DT, int D, int MT, int ST>
-__global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedArgs g) {
-    constexpr int ROWS = 16 * MT;
+// MT tiles of 16 query rows, NW warps, ST ring slots a warp, CPS CTAs per SM.  CUT: the item list is shared out step
+// by step and items are cut; else a CTA takes every gridDim.x-th (request, key head) pair whole.
+template <int DT, int D, int MT, int NW, int ST, int CPS, bool CUT>
+__global__ void __launch_bounds__(32 * NW, CPS) paged_rows_kernel(const PagedArgs g) {
+    constexpr int ROWS = 16 * MT, kThreads = 32 * NW, kKeys = 16 * NW;
     using TL = PackedRows<ROWS, kKeys>;
     constexpr int CH = D / 8;                // 16-byte chunks per key
     constexpr uint32_t kTile = 16 * D * 2;   // one warp's K or V tile
     constexpr int KD = D / 16, ND = D / 8;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(16) long long scratch[34 + (sizeof(WorkPos) + 7) / 8];
-    __shared__ float sm[4][ROWS], sl[4][ROWS];
+    __shared__ WorkShare share;
+    __shared__ float sm[NW][ROWS], sl[NW][ROWS];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t ring = smem_u32(smem) + (uint32_t)warp * ST * 2 * kTile;
-    if (tid == 0 && !g.whole) g.meta[blockIdx.x].last = -1;
     WorkPos w;
-    if (!find_work<TL>(g, w, scratch)) return;
-    ReqView v = request_view(g, w.req);
+    ReqView v;
     const int page_mask = (1 << g.page_shift) - 1;
-
-    while (w.left > 0) {
-        const int steps = TL::steps(g, v, w.tile);
-        const int take = (int)min((long long)(steps - w.step), w.left);
-        int s0 = w.step, s1 = s0 + take;
-        if (g.whole) {  // an item belongs to the CTA that its first step falls to
-            s1 = s0 == 0 ? steps : s0;
-            s0 = s0 == 0 ? 0 : s1;
+    int part_no = 0, n_parts = 0;  // > 0: this CTA has this one part of an item
+    if constexpr (CUT) {
+        constexpr int kRoom = NW * ST * 2 * 16 * D * 2 / 8;
+        const int found = find_part<TL>(g, w, v, part_no, n_parts);
+        if (found < 0) return;
+        if (found == 0) {
+            n_parts = 0;
+            if (!find_work<TL>(g, w, &share, reinterpret_cast<unsigned long long *>(smem), kRoom)) return;
+            v = request_view(g, w.req);
         }
-        if (s1 > s0) {
+    } else {
+        if (blockIdx.x >= (long long)g.B * g.Hkv) return;
+        w.req = (int)(blockIdx.x / (unsigned)g.Hkv), w.head = (int)(blockIdx.x % (unsigned)g.Hkv), w.tile = 0, w.step = 0;
+        v = request_view(g, w.req);
+    }
+
+    while (true) {
+        const int steps = TL::steps(g, v, w.tile);
+        const int s0 = CUT ? w.step : 0, s1 = CUT ? s0 + min(steps - s0, w.left) : steps;
+        if (CUT || v.n > 0) {
             // ---- rows of this thread: lane / 4 (+ 8) of every 16
             int lim[MT][2];
             uint32_t aq[MT][KD][4];
-            const int tok_first = (int)((long long)w.tile * ROWS / g.group);
+            const int tok_first = w.tile == 0 ? 0 : (int)((unsigned long long)w.tile * ROWS / (unsigned)g.group);
             const int lim_first = min(v.shift + tok_first, v.kv - 1);
-            const long long last_row = min((long long)(w.tile + 1) * ROWS, (long long)v.n * g.group) - 1;
-            const int kend = keys_until(v, (int)(last_row / g.group));
+            const int kend = keys_until(v, TL::last_token(g, v, w.tile));
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     int tok, j;
-                    const bool live = TL::place(g, v, w.tile, m * 16 + h * 8 + (lane >> 2), tok, j);
+                    const bool live = TL::place(g, v.n, w.tile, m * 16 + h * 8 + (lane >> 2), tok, j);
                     lim[m][h] = live ? min(v.shift + tok, v.kv - 1) : -1;
                     const char *q = g.q + 2 * (((long long)v.q0 + tok) * g.q_st + (long long)(w.head * g.group + j) * g.q_sh + 2 * (lane & 3));
 #pragma unroll
@@ -311,20 +320,20 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedArgs
             const int row = tid / kPerRow;
             float topw = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) topw = fmaxf(topw, sm[i][row]);
+            for (int i = 0; i < NW; ++i) topw = fmaxf(topw, sm[i][row]);
             const float base = topw == -INFINITY ? 0.f : topw;
-            float wt[4], l = 0.f;
+            float wt[NW], l = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < NW; ++i) {
                 wt[i] = exp2f(sm[i][row] - base);
                 l = fmaf(wt[i], sl[i][row], l);
             }
-            const bool whole_item = s0 == 0 && s1 == steps;
+            const bool whole_item = !CUT || (s0 == 0 && s1 == steps);
             const bool starts = s0 == 0;
             float *part = g.part + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * kPartFloats<ROWS, D>;
             const float inv = l == 0.f ? 0.f : 1.0f / l;
             int tok, j;
-            const bool live = TL::place(g, v, w.tile, row, tok, j);
+            const bool live = TL::place(g, v.n, w.tile, row, tok, j);
             char *out = g.o + 2 * (((long long)v.q0 + tok) * g.o_st + (long long)(w.head * g.group + j) * g.o_sh);
 #pragma unroll
             for (int n0 = 0; n0 < ND; n0 += kPerRow) {
@@ -332,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedArgs
                 if (n >= ND) break;
                 float acc[8] = {};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < NW; ++i) {
                     const float *src = reinterpret_cast<const float *>(smem + (size_t)i * ST * 2 * kTile) + row * D + ((n ^ (row & 7)) * 8);
                     const float4 x = *reinterpret_cast<const float4 *>(src), y = *reinterpret_cast<const float4 *>(src + 4);
                     acc[0] = fmaf(wt[i], x.x, acc[0]), acc[1] = fmaf(wt[i], x.y, acc[1]);
@@ -351,53 +360,120 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedArgs
                     dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
                 }
             }
-            if (!whole_item) {
-                if (tid % kPerRow == 0) part[(size_t)ROWS * D + row] = topw, part[(size_t)ROWS * D + ROWS + row] = l;
-                if (starts && tid == 0) {
-                    PartialItem it;
-                    it.req = w.req, it.head = w.head, it.tile = w.tile;
-                    it.last = cta_of_step(w, w.base + steps - 1);
-                    g.meta[blockIdx.x] = it;
+            if constexpr (CUT) {
+                if (!whole_item) {
+                    if (tid % kPerRow == 0) part[(size_t)ROWS * D + row] = topw, part[(size_t)ROWS * D + ROWS + row] = l;
+                    // Tell the others, and see whether they have all told: the last one to tell (or two that tell at
+                    // the same time, with the same result) joins.  The flags hold a number of this launch and are
+                    // cleared by whoever joins, so what the workspace held before, or a replay of the same captured
+                    // launch, is not taken for it.
+                    __shared__ int all;
+                    __syncthreads();
+                    int c0 = (int)blockIdx.x - part_no, n = n_parts;
+                    if (n_parts == 0) {
+                        const long long item = share.end - w.left - s0;  // its first step in the list
+                        c0 = cta_of(&share, item), n = cta_of(&share, item + steps - 1) - c0 + 1;
+                    }
+                    auto flag = [&](int i) { return g.flags + (size_t)(c0 + i) * 2 + (i == 0 ? 1 : 0); };
+                    if (warp == 0) {
+                        if (lane == 0) {
+                            __threadfence();
+                            *reinterpret_cast<volatile unsigned long long *>(g.flags + (size_t)blockIdx.x * 2 + (starts ? 1 : 0)) = g.tag;
+                            __threadfence();
+                        }
+                        __syncwarp();
+                        bool there = true;
+                        for (int i = lane; i < n; i += 32) there = there && *reinterpret_cast<volatile unsigned long long *>(flag(i)) == g.tag;
+                        there = __all_sync(0xFFFFFFFFu, there) != 0;
+                        __threadfence();
+                        if (lane == 0) all = there ? 1 : 0;
+                    }
+                    __syncthreads();
+                    if (all) {
+                        auto part_of = [&](int i) { return g.part + ((size_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats<ROWS, D>; };
+                        for (int r = warp; r < ROWS; r += NW) {
+                            int t, jj;
+                            if (!TL::place(g, v.n, w.tile, r, t, jj)) break;
+                            float acc[D / 32], sum;
+                            join_row<ROWS, D, 16>(part_of, n, r, lane, acc, sum);
+                            store_joined<DT, D>(g.o + 2 * (((long long)v.q0 + t) * g.o_st + (long long)(w.head * g.group + jj) * g.o_sh), lane, acc, sum);
+                        }
+                        for (int i = tid; i < n; i += kThreads) *reinterpret_cast<volatile unsigned long long *>(flag(i)) = 0ull;
+                    }
                 }
             }
             __syncthreads();  // the rings and statistics are free again
         }
-        w.left -= take;
-        if (w.left <= 0 || !next_item<TL>(g, w, v)) break;
+        if constexpr (CUT) {
+            w.left -= s1 - s0;
+            if (w.left <= 0 || n_parts > 0 || !next_item<TL>(g, w, v)) break;
+        } else if (++w.tile >= TL::tiles(g, v)) {
+            w.tile = 0;
+            const long long pair = (long long)w.req * g.Hkv + w.head + gridDim.x;
+            if (pair >= (long long)g.B * g.Hkv) break;
+            w.req = (int)(pair / g.Hkv), w.head = (int)(pair % g.Hkv);
+            v = request_view(g, w.req);
+        }
     }
 }
 
-template <int DT, int D, int MT>
-int launch_rows(const PagedArgs &g, int sms, cudaStream_t st) {
-    constexpr int ST = D == 128 ? 3 : 6;
-    constexpr size_t smem = 4ull * ST * 2 * 16 * D * 2;
+template <int DT, int D, int MT, int NW, int ST, int CPS, bool CUT>
+int launch_cfg(const PagedArgs &g, int sms, cudaStream_t st) {
+    constexpr size_t smem = (size_t)NW * ST * 2 * 16 * D * 2;
     static SmemLimitCache configured;
-    if (int rc = ensure_dynamic_smem(paged_rows_kernel<DT, D, MT, ST>, smem, configured)) return rc;
-    const unsigned ctas = 2u * (unsigned)sms;
-    paged_rows_kernel<DT, D, MT, ST><<<ctas, kThreads, smem, st>>>(g);
-    if (cudaError_t e = cudaGetLastError()) return (int)e;
-    return g.whole ? DECA_OK : launch_join<DT, D, PackedRows<16 * MT, kKeys>>(g, ctas, st);
+    if (int rc = ensure_dynamic_smem(paged_rows_kernel<DT, D, MT, NW, ST, CPS, CUT>, smem, configured)) return rc;
+    long long ctas = (long long)CPS * sms;
+    if (!CUT && (long long)g.B * g.Hkv < ctas) ctas = (long long)g.B * g.Hkv;
+    paged_rows_kernel<DT, D, MT, NW, ST, CPS, CUT><<<(unsigned)ctas, 32 * NW, smem, st>>>(g);
+    return (int)cudaGetLastError();
+}
+// Four warps; three ring slots of 16 keys each, and as many CTAs as fit: two (D = 128, or 32 rows, by registers) or
+// four an SM.  Two-warp CTAs (more of them) were slower wherever items are cut: twice the parts to join.
+template <int D, int MT>
+constexpr int kCtasPerSm = D == 64 && MT == 1 ? 4 : 2;
+
+template <int DT, int D, int MT>
+int launch_rows(const PagedArgs &g, bool cut, int sms, cudaStream_t st) {
+    return cut ? launch_cfg<DT, D, MT, 4, 3, kCtasPerSm<D, MT>, true>(g, sms, st)
+               : launch_cfg<DT, D, MT, 4, 3, kCtasPerSm<D, MT>, false>(g, sms, st);
 }
 
 template <int DT>
-int launch_rows_dtype(const PagedArgs &g, int D, int mt, int sms, cudaStream_t st) {
-    if (D == 128) return mt == 1 ? launch_rows<DT, 128, 1>(g, sms, st) : launch_rows<DT, 128, 2>(g, sms, st);
-    return mt == 1 ? launch_rows<DT, 64, 1>(g, sms, st) : launch_rows<DT, 64, 2>(g, sms, st);
+int launch_rows_dtype(const PagedArgs &g, int D, int mt, bool cut, int sms, cudaStream_t st) {
+    if (D == 128) return mt == 1 ? launch_rows<DT, 128, 1>(g, cut, sms, st) : launch_rows<DT, 128, 2>(g, cut, sms, st);
+    return mt == 1 ? launch_rows<DT, 64, 1>(g, cut, sms, st) : launch_rows<DT, 64, 2>(g, cut, sms, st);
+}
+
+size_t flag_bytes(int ctas) { return ((size_t)ctas * 2 * sizeof(unsigned long long) + 255) / 256 * 256; }
+
+// A number that no other launch of any process carries, but for one chance in 2^64 or so.
+unsigned long long launch_tag() {
+    static std::atomic<unsigned long long> next{[] {
+        std::random_device rd;
+        return ((unsigned long long)rd() << 32) ^ (unsigned long long)rd() ^ 0x9E3779B97F4A7C15ull;
+    }()};
+    unsigned long long t = next.fetch_add(0x9E3779B97F4A7C15ull);  // odd: runs through all 2^64 values
+    return t ? t : next.fetch_add(0x9E3779B97F4A7C15ull);          // 0 is a cleared flag
 }
 
 }  // namespace
 
-// bytes of workspace for `mt` tiles of 16 rows: one meta record and two partial results per CTA
+int paged_rows_ctas(int D, int mt, int sms) { return (D == 64 && mt == 1 ? kCtasPerSm<64, 1> : kCtasPerSm<128, 1>) * sms; }
+
+// bytes of workspace for `mt` tiles of 16 rows where items are cut: two flags and two partial results per CTA
 size_t paged_rows_workspace(int D, int mt, int sms) {
-    const size_t ctas = 2 * (size_t)sms, rows = 16 * (size_t)mt;
-    return (ctas * sizeof(PartialItem) + 255) / 256 * 256 + ctas * 2 * (rows * D + 2 * rows) * sizeof(float);
+    const size_t rows = 16 * (size_t)mt, ctas = (size_t)paged_rows_ctas(D, mt, sms);
+    return flag_bytes((int)ctas) + ctas * 2 * (rows * D + 2 * rows) * sizeof(float);
 }
 
-int paged_rows_launch(int dtype, PagedArgs &g, int D, int mt, int sms, void *workspace, cudaStream_t st) {
-    const size_t ctas = 2 * (size_t)sms;
-    g.meta = static_cast<PartialItem *>(workspace);
-    g.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + (ctas * sizeof(PartialItem) + 255) / 256 * 256);
-    return dtype == DECA_F16 ? launch_rows_dtype<DECA_F16>(g, D, mt, sms, st) : launch_rows_dtype<DECA_BF16>(g, D, mt, sms, st);
+int paged_rows_launch(const deca_paged_attn_args &a, PagedArgs &g, int mt, bool cut, int sms, cudaStream_t st) {
+    g.flags = static_cast<unsigned long long *>(a.workspace);
+    g.part = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + flag_bytes(paged_rows_ctas(a.D, mt, sms)));
+    g.max_parts = 32;
+    g.min_steps = 4;
+    if (cut) g.tag = launch_tag();
+    return a.dtype == DECA_F16 ? launch_rows_dtype<DECA_F16>(g, a.D, mt, cut, sms, st)
+                               : launch_rows_dtype<DECA_BF16>(g, a.D, mt, cut, sms, st);
 }
 
 }  // namespace deca

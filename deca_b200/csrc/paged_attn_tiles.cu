@@ -41,7 +41,8 @@ struct Layout {
     static constexpr uint32_t kv = q + 2 * kQBytes;
     static constexpr uint32_t stage = kv + kStages * kKVBytes;
     static constexpr uint32_t notes = stage + kStageBytes;
-    static constexpr uint32_t bars = notes + kNotes + 16;  // 16: flags of the two items' notes
+    static constexpr uint32_t share = notes + kNotes + 16;  // 16: flags of the two items' notes
+    static constexpr uint32_t bars = share + (sizeof(WorkShare) + 15) / 16 * 16;
     static constexpr uint32_t bytes = bars + 8 * (2 * kStages + 11);
     static constexpr size_t smem = 1024 + bytes;
 };
@@ -51,20 +52,19 @@ struct RingPos {
     uint32_t par;
 };
 
-// Exponentials of 32 scores (keys cb0 ..) against the maximum's term: packed to 16 bits, summed in fp32.
-template <int DT, bool MASKED, int EVERY>
-__device__ __forceinline__ void exp_chunk32(const uint32_t (&v)[32], int cb0, int lim, uint64_t sl2x2, uint64_t nmsx2,
-                                            const FaPolyConst &pc, uint64_t (&sum2)[2], uint32_t *pk) {
+// Exponentials of 32 scores against the maximum's term: packed to 16 bits, summed in fp32.  A masked score is -inf;
+// the polynomial share would make 2^-126 of it, hence the selection there.
+template <int DT, int EVERY>
+__device__ __forceinline__ void exp_chunk32(const uint32_t (&v)[32], uint64_t sl2x2, uint64_t nmsx2, const FaPolyConst &pc,
+                                            uint64_t (&sum2)[2], uint32_t *pk) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        float s0 = __uint_as_float(v[2 * i]), s1 = __uint_as_float(v[2 * i + 1]);
-        if constexpr (MASKED) {
-            if (cb0 + 2 * i > lim) s0 = -INFINITY;
-            if (cb0 + 2 * i + 1 > lim) s1 = -INFINITY;
-        }
+        const float s0 = __uint_as_float(v[2 * i]), s1 = __uint_as_float(v[2 * i + 1]);
         float p0, p1;
-        if (!MASKED && EVERY > 0 && i % (EVERY > 0 ? EVERY : 1) == (EVERY > 0 ? EVERY : 1) - 1) {
+        if (EVERY > 0 && i % (EVERY > 0 ? EVERY : 1) == (EVERY > 0 ? EVERY : 1) - 1) {
             fa_exp2_poly_pair(s0, s1, pc, p0, p1);
+            if (v[2 * i] == 0xFF800000u) p0 = 0.f;
+            if (v[2 * i + 1] == 0xFF800000u) p1 = 0.f;
         } else {
             float x0, x1;
             f32x2_unpack(f32x2_fma(f32x2_pack(s0, s1), sl2x2, nmsx2), x0, x1);
@@ -75,24 +75,17 @@ __device__ __forceinline__ void exp_chunk32(const uint32_t (&v)[32], int cb0, in
     }
 }
 
-template <bool MASKED>
-__device__ __forceinline__ float row_max32(const uint32_t (&v)[32], int cb0, int lim) {
+__device__ __forceinline__ float max32(const uint32_t (&v)[32]) {
     float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        float s = __uint_as_float(v[i]);
-        if constexpr (MASKED) {
-            if (cb0 + i > lim) s = -INFINITY;
-        }
-        part[i & 3] = fmaxf(part[i & 3], s);
-    }
+    for (int i = 0; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], __uint_as_float(v[i]));
     return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
 }
 
 // Exponentials of the whole row into registers; returns their sum.  The next 32 columns are on their way from
 // tensor memory while the current ones are processed.
-template <int DT, bool MASKED, int EVERY>
-__device__ __forceinline__ float exp_row(uint32_t tS, int col0, int lim, float sl2, float ms, uint32_t (&pk)[kBc / 2]) {
+template <int DT, int EVERY>
+__device__ __forceinline__ float exp_row(uint32_t tS, float sl2, float ms, uint32_t (&pk)[kBc / 2]) {
     const uint64_t sl2x2 = f32x2_pack(sl2, sl2), nmsx2 = f32x2_pack(-ms, -ms);
     const FaPolyConst pc = {sl2 * (1.0f / 256.0f), 126.0f / 256.0f - ms * (1.0f / 256.0f)};
     uint64_t sum2[2] = {0ull, 0ull};
@@ -102,7 +95,7 @@ __device__ __forceinline__ float exp_row(uint32_t tS, int col0, int lim, float s
 #pragma unroll
     for (int c = 0; c < kBc / 32; ++c) {
         if (c + 1 < kBc / 32) tmem_ld_32x32b_x32(tS + (c + 1) * 32, v[(c + 1) & 1]);
-        exp_chunk32<DT, MASKED, EVERY>(v[c & 1], col0 + c * 32, lim, sl2x2, nmsx2, pc, sum2, &pk[c * 16]);
+        exp_chunk32<DT, EVERY>(v[c & 1], sl2x2, nmsx2, pc, sum2, &pk[c * 16]);
         if (c + 1 < kBc / 32) tmem_ld_wait_regs(v[(c + 1) & 1]);
     }
     float a0, a1, b0, b1;
@@ -111,29 +104,48 @@ __device__ __forceinline__ float exp_row(uint32_t tS, int col0, int lim, float s
     return (a0 + a1) + (b0 + b1);
 }
 
+// Puts -inf where the row does not see the key: `visible` leading columns of the tile stay.
+__device__ __forceinline__ void mask_tile(uint32_t tS, int visible) {
+#pragma unroll 1
+    for (int c = 0; c < kBc / 32; ++c) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tS + c * 32, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (c * 32 + i >= visible) v[i] = 0xFF800000u;
+        tmem_st_32x32b_x32(tS + c * 32, v);
+    }
+    tmem_st_wait();
+}
+
 // One key tile of the online softmax for this thread's row.  A row sees a prefix of the keys, so one that
 // sees nothing of a segment's first 32 keys sees nothing of it: m stays -inf, l and P zero.
-template <int DT, int D, bool MASKED>
-__device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, int col0, int lim, float sl2, bool first, float &m,
-                                             float &l) {
-    constexpr int EVERY = kFaPolyEveryFor<D>;
+// There is one copy of the exponentials' code for both passes, and masked tiles are masked in place before it: the
+// warps' roles share the instruction cache, and what falls out of it costs an item microseconds when it ends
+// (with a copy for each case 4 us from the last product of an item to the first score of the next).
+template <int DT, int D>
+__device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, float sl2, bool first, float &m, float &l) {
     if (first) {
         uint32_t v[32];
         tmem_ld_32x32b_x32(tS, v);
         tmem_ld_wait();
-        m = row_max32<MASKED>(v, col0, lim);
+        m = max32(v);
     }
     uint32_t pk[kBc / 2];
-    // held in registers until the vote: storing P overwrites the scores that a second pass would need
-    float sum = exp_row<DT, MASKED, EVERY>(tS, col0, lim, sl2, m == -INFINITY ? 0.f : m * sl2, pk);
-    if (__any_sync(0xFFFFFFFFu, !(sum <= kFaSumLimit))) {
+    float sum;
+#pragma unroll 1
+    for (bool again = false;; again = true) {
+        // held in registers until the vote: storing P overwrites the scores that a second pass would need
+        sum = exp_row<DT, kFaPolyEveryFor<D>>(tS, sl2, m == -INFINITY ? 0.f : m * sl2, pk);
+        if (again || !__any_sync(0xFFFFFFFFu, !(sum <= kFaSumLimit))) break;
         float top = m;
 #pragma unroll 1
         for (int c = 0; c < kBc / 32; ++c) {
             uint32_t v[32];
             tmem_ld_32x32b_x32(tS + c * 32, v);
             tmem_ld_wait();
-            top = fmaxf(top, row_max32<MASKED>(v, col0 + c * 32, lim));
+            top = fmaxf(top, max32(v));
         }
         const float alpha = m == -INFINITY ? 0.f : ex2_approx((m - top) * sl2);
         l *= alpha;
@@ -151,7 +163,6 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, int col0,
             }
             tmem_st_wait();
         }
-        sum = exp_row<DT, MASKED, 0>(tS, col0, lim, sl2, m == -INFINITY ? 0.f : m * sl2, pk);
     }
     l += sum;
 #pragma unroll
@@ -164,10 +175,10 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, int col0,
     tmem_st_wait();
 }
 
+// Bit 15 or 31 is set where that half of a packed pair is an infinity or a NaN (other bits are noise).
 template <int DT>
-__device__ __forceinline__ bool word_not_finite(uint32_t w) {
-    constexpr uint32_t e = DT == DECA_F16 ? 0x7C00u : 0x7F80u;
-    return (w & e) == e || ((w >> 16) & e) == e;
+__device__ __forceinline__ uint32_t exponent_carry(uint32_t w) {
+    return DT == DECA_F16 ? (w & 0x7C007C00u) + 0x04000400u : (w & 0x7F807F80u) + 0x00800080u;
 }
 
 template <int DT, int D>
@@ -204,7 +215,10 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 
     if (threadIdx.x == 0) g.meta[blockIdx.x].last = -1;
     WorkPos w;
-    if (!find_work<TL>(g, w, reinterpret_cast<long long *>(smem + L::stage))) return;  // the whole CTA leaves
+    allow_next_kernel();
+    WorkShare *share = reinterpret_cast<WorkShare *>(smem + L::share);
+    // the ring is free for the costs
+    if (!find_work<TL>(g, w, share, reinterpret_cast<unsigned long long *>(smem + L::kv), (int)(kStages * L::kKVBytes / 8))) return;
     ReqView v = request_view(g, w.req);
 
     // rows of the Q tiles that no token reaches stay zero
@@ -253,7 +267,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     };
     auto segment = [&](int &steps) {  // steps of the current item that are this CTA's
         steps = TL::steps(g, v, w.tile);
-        return (int)min((long long)(steps - w.step), w.left);
+        return min(steps - w.step, w.left);
     };
     auto next = [&](int n) {
         w.left -= n;
@@ -337,29 +351,11 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (lane == 0) {
             constexpr uint64_t kDescK = (uint64_t(16 >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
             constexpr uint64_t kDescV = (uint64_t((kKVBlock >> 4) & 0x3FFF) << 16) | (uint64_t(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-            const uint64_t q_desc[2] = {kDescK | (uint64_t)((sQ & 0x3FFFFu) >> 4),
-                                        kDescK | (uint64_t)(((sQ + L::kQBytes) & 0x3FFFFu) >> 4)};
-            auto issue_qk = [&](int grp, const RingPos &kp) {  // S_grp = Q_grp K^T
-                const uint64_t kdesc = kDescK | (uint64_t)(((sKV + kp.slot * L::kKVBytes) & 0x3FFFFu) >> 4);
-                const uint32_t d_tmem = tS(grp);
-#pragma unroll
-                for (int kd = 0; kd < D / 16; ++kd)
-                    umma_f16_ss(d_tmem, q_desc[grp] + (((kd / 4) * 16384 + (kd % 4) * 32) >> 4),
-                                kdesc + (((kd / 4) * kKVBlock + (kd % 4) * 32) >> 4), kIdescQK, kd != 0 ? 1u : 0u);
-                umma_commit(s_full(grp));
-            };
-            auto issue_pv = [&](int grp, const RingPos &vp, uint32_t first, bool last) {  // O_grp (+)= P_grp V
-                const uint64_t vdesc = kDescV | (uint64_t)(((sKV + vp.slot * L::kKVBytes) & 0x3FFFFu) >> 4);
-                const uint32_t d_tmem = tO(grp), a_tmem = tS(grp);
-#pragma unroll
-                for (int kk = 0; kk < kBc / 16; ++kk)
-                    umma_f16_ts(d_tmem, a_tmem + kk * 8, vdesc + kk * (2048 >> 4), kIdescPV, (first | kk) != 0 ? 1u : 0u);
-                if (last) umma_commit(pv_done(grp));  // the segment's O_grp is complete
-            };
+            const uint64_t q_desc = kDescK | (uint64_t)((sQ & 0x3FFFFu) >> 4);
             RingPos kp{0, 0u}, vp{1, 0u};
             uint32_t cnt = 0;  // key tiles handled so far
             int n_local = 0;
-            while (true) {
+            while (ok) {
                 int steps;
                 const int n = segment(steps);
                 if (!mbar_wait(q_full, (uint32_t)(n_local & 1), abort_flag) || !mbar_wait(kv_full(kp.slot), kp.par, abort_flag)) {
@@ -367,37 +363,45 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     ok = false;
                     break;
                 }
-                tc_fence_after_sync();
-                issue_qk(0, kp);
-                issue_qk(1, kp);
-                umma_commit(kv_empty(kp.slot));
-                if (n == 1) umma_commit(q_free);  // that was the segment's last score MMA
-                advance(kp, 2);
-                for (int j = 0; j < n; ++j) {
-                    // V_j and K_{j+1} have landed once p_full completes: the relay arrives there after them
-                    if (!mbar_wait(p_full(0), (cnt + (uint32_t)j) & 1u, abort_flag)) {
-                        report_detail(g.status, 1, 5, j);
-                        ok = false;
-                        break;
+                // round j: the products of tile j (none in round -1) and the scores of tile j + 1
+#pragma unroll 1
+                for (int j = -1; j < n && ok; ++j) {
+                    const uint64_t kdesc = kDescK | (uint64_t)(((sKV + kp.slot * L::kKVBytes) & 0x3FFFFu) >> 4);
+                    const uint64_t vdesc = kDescV | (uint64_t)(((sKV + vp.slot * L::kKVBytes) & 0x3FFFFu) >> 4);
+#pragma unroll 1
+                    for (int grp = 0; grp < 2; ++grp) {
+                        const uint32_t s_tmem = tS(grp), o_tmem = tO(grp);
+                        if (j >= 0) {
+                            // V_j and K_{j+1} have landed once p_full completes: the relay arrives there after them
+                            if (!mbar_wait(p_full(grp), (cnt + (uint32_t)j) & 1u, abort_flag)) {
+                                report_detail(g.status, 1, 5 + grp, j);
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after_sync();
+#pragma unroll
+                            for (int kk = 0; kk < kBc / 16; ++kk)  // O_grp (+)= P_grp V
+                                umma_f16_ts(o_tmem, s_tmem + kk * 8, vdesc + kk * (2048 >> 4), kIdescPV, (j | kk) != 0 ? 1u : 0u);
+                            if (j + 1 == n) umma_commit(pv_done(grp));  // the segment's O_grp is complete
+                            if (grp == 1) umma_commit(kv_empty(vp.slot));
+                        } else {
+                            tc_fence_after_sync();
+                        }
+                        if (j + 1 < n) {
+                            const uint64_t qd = q_desc + grp * (L::kQBytes >> 4);
+#pragma unroll
+                            for (int kd = 0; kd < D / 16; ++kd)  // S_grp = Q_grp K^T
+                                umma_f16_ss(s_tmem, qd + (((kd / 4) * 16384 + (kd % 4) * 32) >> 4),
+                                            kdesc + (((kd / 4) * kKVBlock + (kd % 4) * 32) >> 4), kIdescQK, kd != 0 ? 1u : 0u);
+                            umma_commit(s_full(grp));
+                            if (grp == 1) {
+                                umma_commit(kv_empty(kp.slot));
+                                if (j + 2 == n) umma_commit(q_free);  // the segment's last score MMA
+                            }
+                        }
                     }
-                    tc_fence_after_sync();
-                    issue_pv(0, vp, (uint32_t)j, j + 1 == n);
-                    if (j + 1 < n) issue_qk(0, kp);
-                    if (!mbar_wait(p_full(1), (cnt + (uint32_t)j) & 1u, abort_flag)) {
-                        report_detail(g.status, 1, 6, j);
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after_sync();
-                    issue_pv(1, vp, (uint32_t)j, j + 1 == n);
-                    umma_commit(kv_empty(vp.slot));
-                    if (j + 1 < n) {
-                        issue_qk(1, kp);
-                        umma_commit(kv_empty(kp.slot));
-                        if (j + 2 == n) umma_commit(q_free);  // the segment's last score MMA
-                        advance(kp, 2);
-                    }
-                    advance(vp, 2);
+                    if (j >= 0) advance(vp, 2);
+                    if (j + 1 < n) advance(kp, 2);
                 }
                 cnt += (uint32_t)n;
                 ++n_local;
@@ -449,14 +453,18 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 if (key0 + kBc - 1 > common) {
                     uint8_t *tile = smem + L::kv + vp.slot * L::kKVBytes;
                     const int r0 = min(max(common + 1 - key0, 0), kBc), r1 = min(max(kend - key0, 0), kBc);
-                    bool bad = false;
-                    for (int i = r0 * 8 + lane; i < r1 * 8; i += 32)
+                    // an exponent of ones carries into the sign's place; eight loads are in flight
+                    uint32_t seen = 0;
+                    for (int i0 = r0 * 8 + lane; i0 < r1 * 8; i0 += 32 * 8 / (D / 64))
 #pragma unroll
-                        for (int b = 0; b < D / 64; ++b) {
-                            const uint4 x = *reinterpret_cast<const uint4 *>(tile + b * kKVBlock + i * 16);
-                            bad = bad || word_not_finite<DT>(x.x) || word_not_finite<DT>(x.y) || word_not_finite<DT>(x.z) ||
-                                  word_not_finite<DT>(x.w);
-                        }
+                        for (int k = 0; k < 8 / (D / 64); ++k)
+#pragma unroll
+                            for (int b = 0; b < D / 64; ++b) {
+                                const int i = i0 + 32 * k;
+                                const uint4 x = i < r1 * 8 ? *reinterpret_cast<const uint4 *>(tile + b * kKVBlock + i * 16) : make_uint4(0, 0, 0, 0);
+                                seen |= exponent_carry<DT>(x.x) | exponent_carry<DT>(x.y) | exponent_carry<DT>(x.z) | exponent_carry<DT>(x.w);
+                            }
+                    const bool bad = (seen & 0x80008000u) != 0;
                     for (int i = r1 * 8 + lane; i < kBc * 8; i += 32)
 #pragma unroll
                         for (int b = 0; b < D / 64; ++b)
@@ -511,7 +519,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             int kend, common;
             item_keys(kend, common);
             int tok, head;
-            const bool live = TL::place(g, v, w.tile, grp * kBr + r, tok, head);
+            const bool live = TL::place(g, v.n, w.tile, grp * kBr + r, tok, head);
             const int lim = live ? min(v.shift + tok, v.kv - 1) : -1;
             const int lim_tile = min(v.shift + min((2 * w.tile + grp) * tpt, v.n), v.kv - 1);  // of the tile's first row
             float m = -INFINITY, l = 0.f;
@@ -523,10 +531,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
                 tc_fence_after_sync();
                 const int col0 = (w.step + j) * kBc;
-                if (col0 + kBc - 1 > lim_tile)
-                    softmax_tile<DT, D, true>(tSg, tOg, col0, lim, sl2, j == 0, m, l);
-                else
-                    softmax_tile<DT, D, false>(tSg, tOg, col0, lim, sl2, j == 0, m, l);
+                if (col0 + kBc - 1 > lim_tile) mask_tile(tSg, lim + 1 - col0);
+                softmax_tile<DT, D>(tSg, tOg, sl2, j == 0, m, l);
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full(grp));
@@ -542,20 +548,27 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             // ---- epilogue: through this warp's panel, so that eight lanes write 128 bytes of a row
             const bool whole = n == steps;
             const float inv = l == 0.f ? 0.f : 1.0f / l;
-            const bool fix = noted[item & 1] != 0;
-            const uint8_t *note = notes + (item & 1) * 3 * D;
-            auto value = [&](uint32_t x, int d) {  // numerator of column d, with what was taken out of V
-                float f = __uint_as_float(x);
-                if (fix) {
-                    const int seen = lim - common - 1;
-                    const bool up = note[D + d] <= seen, down = note[2 * D + d] <= seen;
-                    if (note[d] <= seen || (up && down))
-                        f = __int_as_float(0x7FC00000);
-                    else if (up || down)
-                        f = up ? INFINITY : -INFINITY;
+            if (noted[item & 1] != 0) {
+                // what was taken out of V goes to the rows that see it
+                const uint8_t *note = notes + (item & 1) * 3 * D;
+                const int seen = lim - common - 1;
+#pragma unroll 1
+                for (int b = 0; b < D / 32; ++b) {
+                    uint32_t x[32];
+                    tmem_ld_32x32b_x32(tOg + b * 32, x);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const uint8_t *at = note + b * 32 + i;
+                        const bool up = at[D] <= seen, down = at[2 * D] <= seen;
+                        if (up) x[i] = 0x7F800000u;
+                        if (down) x[i] = 0xFF800000u;
+                        if (at[0] <= seen || (up && down)) x[i] = 0x7FC00000u;
+                    }
+                    tmem_st_32x32b_x32(tOg + b * 32, x);
                 }
-                return f;
-            };
+                tmem_st_wait();
+            }
             const int sub = lane >> 3, c8 = lane & 7;  // row within four, 16-byte chunk
             const uint32_t live_rows = __ballot_sync(0xFFFFFFFFu, live);
             if (whole) {
@@ -573,7 +586,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         uint32_t o[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            o[i] = Pack16<DT>::pack(value(x[2 * i], b * 64 + c * 8 + 2 * i) * inv, value(x[2 * i + 1], b * 64 + c * 8 + 2 * i + 1) * inv);
+                            o[i] = Pack16<DT>::pack(__uint_as_float(x[2 * i]) * inv, __uint_as_float(x[2 * i + 1]) * inv);
                         *reinterpret_cast<uint4 *>(panel + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
                     }
                     __syncwarp();
@@ -597,9 +610,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     __syncwarp();
 #pragma unroll
                     for (int c = 0; c < 8; ++c)
-                        *reinterpret_cast<float4 *>(panel + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                            make_float4(value(v0[4 * c], b * 32 + 4 * c), value(v0[4 * c + 1], b * 32 + 4 * c + 1),
-                                        value(v0[4 * c + 2], b * 32 + 4 * c + 2), value(v0[4 * c + 3], b * 32 + 4 * c + 3));
+                        *reinterpret_cast<uint4 *>(panel + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                            make_uint4(v0[4 * c], v0[4 * c + 1], v0[4 * c + 2], v0[4 * c + 3]);
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -613,8 +625,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 part[(size_t)TL::ROWS * D + TL::ROWS + grp * kBr + r] = l;
                 if (starts && threadIdx.x == 64) {
                     PartialItem it;
-                    it.req = w.req, it.head = w.head, it.tile = w.tile;
-                    it.last = cta_of_step(w, w.base + steps - 1);
+                    it.last = cta_of(share, share->end + (steps - n) - 1);
+                    it.head = w.head, it.tile = w.tile, it.q0 = v.q0, it.n = v.n;
                     g.meta[blockIdx.x] = it;
                 }
             }
@@ -662,7 +674,7 @@ int launch_tiles(const PagedArgs &g, const deca_paged_attn_args &a, int sms, cud
     if (int rc = ensure_dynamic_smem(paged_tiles_kernel<DT, D>, Layout<D>::smem, configured)) return rc;
     paged_tiles_kernel<DT, D><<<(unsigned)sms, kThreads, Layout<D>::smem, st>>>(tmQ, tmK, tmV, g);
     if (cudaError_t e = cudaGetLastError()) return (int)e;
-    return launch_join<DT, D, TL>(g, (unsigned)sms, st);
+    return launch_join<DT, D, TL>(g, (unsigned)sms, 16, st);
 }
 
 }  // namespace
@@ -672,6 +684,7 @@ size_t paged_tiles_workspace(int D, int sms) {
 }
 
 int paged_tiles_launch(const deca_paged_attn_args &a, PagedArgs &g, int sms, cudaStream_t st) {
+    g.tile_tokens = 128 / g.group;
     g.meta = static_cast<PartialItem *>(a.workspace);
     g.part = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + ((size_t)sms * sizeof(PartialItem) + 255) / 256 * 256);
     if (a.dtype == DECA_F16)

@@ -34,95 +34,110 @@ struct RotArgs {
     float sine;
 };
 
-// V elements, 16 bytes (V = 8) or one element (V = 1)
-template <int DT, int V>
-__device__ __forceinline__ void load_part(float (&f)[V], const char *p) {
-    if constexpr (V == 8) {
-        uint32_t d[4];
+// V elements as they lie in memory: 16 bytes (V = 8) or one element (V = 1)
+template <int V>
+struct Raw;
+template <>
+struct Raw<8> {
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const char *p) {
         asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                      : "l"(p));
+    }
+    __device__ __forceinline__ void store(char *p) const { *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]); }
+    template <int DT>
+    __device__ __forceinline__ void get(float (&f)[8]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float2 x = Pack16<DT>::unpack(d[i]);
+            const float2 x = Pack16<DT>::unpack(w[i]);
             f[2 * i] = x.x, f[2 * i + 1] = x.y;
         }
-    } else if constexpr (DT == DECA_F16) {
-        f[0] = __half2float(*reinterpret_cast<const __half *>(p));
-    } else {
-        f[0] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(p));
     }
-}
-template <int DT, int V>
-__device__ __forceinline__ void store_part(char *p, const float (&f)[V]) {
-    if constexpr (V == 8) {
-        *reinterpret_cast<uint4 *>(p) = make_uint4(Pack16<DT>::pack(f[0], f[1]), Pack16<DT>::pack(f[2], f[3]),
-                                                   Pack16<DT>::pack(f[4], f[5]), Pack16<DT>::pack(f[6], f[7]));
-    } else if constexpr (DT == DECA_F16) {
-        *reinterpret_cast<__half *>(p) = __float2half_rn(f[0]);
-    } else {
-        *reinterpret_cast<__nv_bfloat16 *>(p) = __float2bfloat16_rn(f[0]);
-    }
-}
-
-// One unit of a head is two parts of V elements: unit u < rot / 2V holds V whole pairs, the others lie
-// behind the rotated elements.
-template <int DT, int V, int LAYOUT>
-struct Unit {
-    float a[V], b[V];
-    static __device__ __forceinline__ int off_a(int u, int rot) {
-        return (LAYOUT == DECA_ROT_HALF && u * 2 * V < rot) ? u * V : u * 2 * V;
-    }
-    static __device__ __forceinline__ int off_b(int u, int rot) {
-        return (LAYOUT == DECA_ROT_HALF && u * 2 * V < rot) ? u * V + rot / 2 : u * 2 * V + V;
-    }
-    __device__ __forceinline__ void load(const char *head, int u, int rot) {
-        load_part<DT, V>(a, head + 2 * off_a(u, rot));
-        load_part<DT, V>(b, head + 2 * off_b(u, rot));
-    }
-    __device__ __forceinline__ void store(char *head, int u, int rot) const {
-        store_part<DT, V>(head + 2 * off_a(u, rot), a);
-        store_part<DT, V>(head + 2 * off_b(u, rot), b);
-    }
-    __device__ __forceinline__ void turn(const float2 *cs, int u) {
-        if constexpr (LAYOUT == DECA_ROT_HALF || V == 1) {
+    template <int DT>
+    __device__ __forceinline__ void set(const float (&f)[8]) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float2 w = cs[u * V + i];
-                const float x = a[i], y = b[i];
-                a[i] = x * w.x - y * w.y;
-                b[i] = x * w.y + y * w.x;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; i += 2) {  // pairs lie side by side within a part
-                float2 w = cs[u * V + i / 2];
-                float x = a[i], y = a[i + 1];
-                a[i] = x * w.x - y * w.y;
-                a[i + 1] = x * w.y + y * w.x;
-                w = cs[u * V + V / 2 + i / 2];
-                x = b[i], y = b[i + 1];
-                b[i] = x * w.x - y * w.y;
-                b[i + 1] = x * w.y + y * w.x;
-            }
-        }
+        for (int i = 0; i < 4; ++i) w[i] = Pack16<DT>::pack(f[2 * i], f[2 * i + 1]);
     }
 };
+template <>
+struct Raw<1> {
+    uint16_t w;
+    __device__ __forceinline__ void load(const char *p) { w = *reinterpret_cast<const uint16_t *>(p); }
+    __device__ __forceinline__ void store(char *p) const { *reinterpret_cast<uint16_t *>(p) = w; }
+    template <int DT>
+    __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = Pack16<DT>::unpack(w).x; }
+    template <int DT>
+    __device__ __forceinline__ void set(const float (&f)[1]) { w = (uint16_t)Pack16<DT>::pack(f[0], 0.f); }
+};
 
+// Turns the pairs of one unit; cs: the first of its V angles.
+template <int DT, int V, int LAYOUT>
+__device__ __forceinline__ void turn(Raw<V> &ra, Raw<V> &rb, const float2 *cs) {
+    float a[V], b[V];
+    ra.template get<DT>(a);
+    rb.template get<DT>(b);
+    if constexpr (LAYOUT == DECA_ROT_HALF || V == 1) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float2 w = cs[i];
+            const float x = a[i], y = b[i];
+            a[i] = x * w.x - y * w.y;
+            b[i] = x * w.y + y * w.x;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {  // pairs lie side by side within a part
+            float2 w = cs[i / 2];
+            float x = a[i], y = a[i + 1];
+            a[i] = x * w.x - y * w.y;
+            a[i + 1] = x * w.y + y * w.x;
+            w = cs[V / 2 + i / 2];
+            x = b[i], y = b[i + 1];
+            b[i] = x * w.x - y * w.y;
+            b[i + 1] = x * w.y + y * w.x;
+        }
+    }
+    ra.template set<DT>(a);
+    rb.template set<DT>(b);
+}
+
+constexpr int kUnits = 4;  // units of a thread whose loads are issued together
+
+// One CTA per token (or share of its heads, gridDim.y of them).  A unit is two parts of V elements of a head:
+// V whole pairs, or 2 V elements behind the rotated ones; a thread keeps its place within the head and
+// walks over the heads of q, then k, then v, so it needs one division.  Its first units are on their way
+// while the angles are computed.
 template <int DT, int V, int LAYOUT>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotArgs g, const __grid_constant__ Turns turns) {
     __shared__ float2 cs[kMaxPairs];
-    using U = Unit<DT, V, LAYOUT>;
     const long long tok = blockIdx.x;
     const int per_head = g.D / (2 * V);
-    const int n_units = (g.Hq + 2 * g.Hkv) * per_head;
-    const int step = kThreads * gridDim.y;
-    int i = blockIdx.y * kThreads + threadIdx.x;
+    const int at = blockIdx.y * blockDim.x + threadIdx.x;  // blockDim.x is a multiple of per_head
+    const int u = at % per_head, step = (int)(blockDim.x * gridDim.y) / per_head;
+    const bool rotated = u * 2 * V < g.rot;
+    const bool split = LAYOUT == DECA_ROT_HALF && rotated;
+    const int off_a = split ? u * V : u * 2 * V, off_b = split ? u * V + g.rot / 2 : u * 2 * V + V;
+    const int heads = g.Hq + 2 * g.Hkv;
 
-    const char *src = nullptr;
-    char *dst = nullptr;
-    int u = 0;
-    bool rotate = false;
+    auto source = [&](int head) -> const char * {
+        if (head < g.Hq) return g.q + 2 * (tok * g.q_st + head * g.q_sh);
+        head -= g.Hq;
+        if (head < g.Hkv) return g.k + 2 * (tok * g.k_st + head * g.k_sh);
+        return g.v + 2 * (tok * g.v_st + (head - g.Hkv) * g.v_sh);
+    };
+    Raw<V> a[kUnits], b[kUnits];
+    int head = at / per_head;
+    auto load = [&]() {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i)
+            if (head + i * step < heads) {
+                const char *src = source(head + i * step);
+                a[i].load(src + 2 * off_a);
+                b[i].load(src + 2 * off_b);
+            }
+    };
+    load();
     long long row_k = -1, row_v = -1;  // element offsets of the token's cache rows, -1: none
     if (g.Hkv > 0) {
         const long long slot = g.slots[tok];
@@ -132,49 +147,36 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotArgs g, const
             row_v = page * g.vc_sp + row * g.vc_sr;
         }
     }
-    auto place = [&](int idx) {  // unit idx of the token: heads of q, then k, then v
-        int head = idx / per_head;
-        u = idx - head * per_head;
-        rotate = u * 2 * V < g.rot;
-        if (head < g.Hq) {
-            src = g.q + 2 * (tok * g.q_st + head * g.q_sh);
-            dst = g.qo + 2 * (tok * g.qo_st + head * g.qo_sh);
-            return;
-        }
-        head -= g.Hq;
-        if (head < g.Hkv) {
-            src = g.k + 2 * (tok * g.k_st + head * g.k_sh);
-            dst = row_k >= 0 ? g.kc + 2 * (row_k + head * g.kc_sh) : nullptr;
-        } else {
-            head -= g.Hkv;
-            src = g.v + 2 * (tok * g.v_st + head * g.v_sh);
-            dst = row_v >= 0 ? g.vc + 2 * (row_v + head * g.vc_sh) : nullptr;
-            rotate = false;
-        }
-    };
-    // the first unit's loads are in flight while the angles are computed.  A v unit is copied, so its
-    // parts need not follow the pairing of the rotation
-    U x;
-    if (i < n_units) {
-        place(i);
-        x.load(src, u, g.rot);
-    }
     const long long pos = g.positions[tok];
-    for (int p = threadIdx.x; p < g.rot / 2; p += kThreads) {
+    for (int p = threadIdx.x; p < g.rot / 2; p += blockDim.x) {
         const long long angle = (long long)((unsigned long long)pos * turns.t[p]);  // 2^63 = half a turn
         float s, c;
         sincospif((float)angle * 1.0842021724855044e-19f, &s, &c);
         cs[p] = make_float2(c * g.amplitude, s * g.sine);
     }
     __syncthreads();
-    while (i < n_units) {
-        if (rotate) x.turn(cs, u);
-        if (dst) x.store(dst, u, g.rot);
-        i += step;
-        if (i < n_units) {
-            place(i);
-            x.load(src, u, g.rot);
+    while (true) {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            int h = head + i * step;
+            if (h >= heads) break;
+            char *dst;
+            if (h < g.Hq) {
+                dst = g.qo + 2 * (tok * g.qo_st + h * g.qo_sh);
+            } else if ((h -= g.Hq) < g.Hkv) {
+                dst = row_k >= 0 ? g.kc + 2 * (row_k + h * g.kc_sh) : nullptr;
+            } else {
+                dst = row_v >= 0 ? g.vc + 2 * (row_v + (h - g.Hkv) * g.vc_sh) : nullptr;
+            }
+            if (rotated && head + i * step < g.Hq + g.Hkv) turn<DT, V, LAYOUT>(a[i], b[i], cs + u * V);
+            if (dst) {
+                a[i].store(dst + 2 * off_a);
+                b[i].store(dst + 2 * off_b);
+            }
         }
+        head += kUnits * step;
+        if (head >= heads) return;
+        load();
     }
 }
 
@@ -195,11 +197,11 @@ bool vector_ok(const deca_cache *c) {
 }
 
 template <int DT, int V>
-void launch_layout(const RotArgs &g, const Turns &t, int layout, dim3 grid, cudaStream_t st) {
+void launch_layout(const RotArgs &g, const Turns &t, int layout, dim3 grid, unsigned threads, cudaStream_t st) {
     if (layout == DECA_ROT_HALF)
-        rotary_kernel<DT, V, DECA_ROT_HALF><<<grid, kThreads, 0, st>>>(g, t);
+        rotary_kernel<DT, V, DECA_ROT_HALF><<<grid, threads, 0, st>>>(g, t);
     else
-        rotary_kernel<DT, V, DECA_ROT_INTERLEAVED><<<grid, kThreads, 0, st>>>(g, t);
+        rotary_kernel<DT, V, DECA_ROT_INTERLEAVED><<<grid, threads, 0, st>>>(g, t);
 }
 
 int launch_rotary(int dtype, RotArgs &g, const deca_rotation *r, long long tokens, bool vec, cudaStream_t st) {
@@ -211,15 +213,23 @@ int launch_rotary(int dtype, RotArgs &g, const deca_rotation *r, long long token
     Turns t;
     for (int i = 0; i < r->rot_dim / 2; ++i) t.t[i] = r->turns[i];
     for (int i = r->rot_dim / 2; i < kMaxPairs; ++i) t.t[i] = 0;
-    // few tokens: the units of a token are shared by several CTAs
-    const int units = (g.Hq + 2 * g.Hkv) * (r->D / (vec ? 16 : 2));
+    const int per_head = r->D / (vec ? 16 : 2);
+    const int heads = g.Hq + 2 * g.Hkv;
+    // Threads: as few groups of a head's units as cover the heads in whole rounds, about `want` units each
+    const int most = kThreads / per_head;  // heads that a CTA of full size takes at once
+    const int want = tokens < 296 ? 1 : 3;
+    int at_once = (heads + want - 1) / want;
+    if (at_once * per_head < 64) at_once = (63 + per_head) / per_head;  // the angles want two warps
+    if (at_once > most) at_once = most;
+    // few tokens: the heads of a token are shared by several CTAs
     int split = 1;
-    while (tokens * split < 296 && split * kThreads < units && split < 64) split *= 2;
+    while (tokens * split < 296 && split * at_once < heads && split < 64) split *= 2;
     const dim3 grid((unsigned)tokens, (unsigned)split);
+    const unsigned threads = (unsigned)(at_once * per_head);
     if (dtype == DECA_F16)
-        vec ? launch_layout<DECA_F16, 8>(g, t, r->layout, grid, st) : launch_layout<DECA_F16, 1>(g, t, r->layout, grid, st);
+        vec ? launch_layout<DECA_F16, 8>(g, t, r->layout, grid, threads, st) : launch_layout<DECA_F16, 1>(g, t, r->layout, grid, threads, st);
     else
-        vec ? launch_layout<DECA_BF16, 8>(g, t, r->layout, grid, st) : launch_layout<DECA_BF16, 1>(g, t, r->layout, grid, st);
+        vec ? launch_layout<DECA_BF16, 8>(g, t, r->layout, grid, threads, st) : launch_layout<DECA_BF16, 1>(g, t, r->layout, grid, threads, st);
     return (int)cudaGetLastError();
 }
 
