@@ -96,6 +96,25 @@ at::Tensor fresh(at::IntArrayRef shape, at::ScalarType dtype, int device) {
     return at::detail::empty_cuda(shape, dtype, c10::Device(c10::kCUDA, (c10::DeviceIndex)device), std::nullopt);
 }
 
+// Several one-dimensional tensors in one allocation, each on a boundary of 256 bytes: an allocation costs the host
+// about as much as a launch.
+struct Shared {
+    int64_t bytes = 0;
+    at::Tensor buffer;
+    int64_t reserve(int64_t count, int64_t size) {
+        const int64_t at = bytes;
+        bytes += (count * size + 255) / 256 * 256;
+        return at;
+    }
+    at::Tensor tensor(int64_t at, int64_t count, at::ScalarType dtype) const {
+        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), c10::scalarTypeToTypeMeta(dtype));
+        c10::TensorImpl *impl = t.unsafeGetTensorImpl();
+        impl->set_sizes_contiguous({count});
+        impl->set_storage_offset(at / (int64_t)c10::elementSize(dtype));
+        return t;
+    }
+};
+
 // An output: the caller's tensor, or a new contiguous one.
 at::Tensor output(PyObject *const *args, Py_ssize_t n, Py_ssize_t i, const char *name, at::ScalarType dtype, at::IntArrayRef shape, int device) {
     if (given(args, n, i)) return view(args[i], name, dtype, shape, device);
@@ -329,9 +348,19 @@ PyObject *paged_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
         const int64_t stride = p.B > 1 ? table.stride(0) : p.W;
         if (stride < p.W) refuse("block_table: rows overlap");
         if (pages.size(0) > 2147483647ll) refuse("free_pages: more than 2^31 - 1 entries");
-        at::Tensor cu = output(args, n, 6, "cu_q", at::kInt, {p.B + 1}, dev), kv = output(args, n, 7, "kv_lens", at::kInt, {p.B}, dev);
-        at::Tensor pos = output(args, n, 8, "positions", at::kInt, {p.T}, dev), slots = output(args, n, 9, "slots", at::kLong, {p.T}, dev);
-        at::Tensor left = output(args, n, 10, "n_free_out", at::kInt, {1}, dev), missing = output(args, n, 11, "short", at::kInt, {1}, dev);
+        at::Tensor cu, kv, pos, slots, left, missing;
+        if (n <= 6) {
+            Shared all;
+            const int64_t a = all.reserve(p.B + 1, 4), b = all.reserve(p.B, 4), c = all.reserve(p.T, 4), d = all.reserve(p.T, 8),
+                          e = all.reserve(1, 4), f = all.reserve(1, 4);
+            all.buffer = fresh({all.bytes}, at::kByte, dev);
+            cu = all.tensor(a, p.B + 1, at::kInt), kv = all.tensor(b, p.B, at::kInt), pos = all.tensor(c, p.T, at::kInt);
+            slots = all.tensor(d, p.T, at::kLong), left = all.tensor(e, 1, at::kInt), missing = all.tensor(f, 1, at::kInt);
+        } else {
+            cu = output(args, n, 6, "cu_q", at::kInt, {p.B + 1}, dev), kv = output(args, n, 7, "kv_lens", at::kInt, {p.B}, dev);
+            pos = output(args, n, 8, "positions", at::kInt, {p.T}, dev), slots = output(args, n, 9, "slots", at::kLong, {p.T}, dev);
+            left = output(args, n, 10, "n_free_out", at::kInt, {1}, dev), missing = output(args, n, 11, "short", at::kInt, {1}, dev);
+        }
         check_status(deca_paged_step(ctx.data_ptr<int32_t>(), add.data_ptr<int32_t>(), p.B, table.data_ptr<int32_t>(), stride, p.W,
                                      pages.data_ptr<int32_t>(), (int)pages.size(0), n_free.data_ptr<int32_t>(), p.page_size, p.T,
                                      cu.data_ptr<int32_t>(), kv.data_ptr<int32_t>(), pos.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),

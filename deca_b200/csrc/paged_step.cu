@@ -13,7 +13,8 @@
 namespace deca {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRequests = 8192;
 
 struct StepArgs {
@@ -69,7 +70,8 @@ __global__ void __launch_bounds__(kThreads) paged_step_kernel(const StepArgs g) 
     int *tok = smem;                // [B] first token of each request
     int *pages = smem + g.B;        // [B] first of its new pages in the order of the step
     int *ctx_of = smem + 2 * g.B;   // [B]
-    __shared__ int warp_tok[32], warp_pages[32];
+    __shared__ int warp_tok[kWarps], warp_pages[kWarps];
+    const int free_given = *g.n_free;  // on its way while the lengths are summed
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (g.B + kThreads - 1) / kThreads;
     const int r0 = min(tid * per, g.B), r1 = min(r0 + per, g.B);
@@ -94,15 +96,20 @@ __global__ void __launch_bounds__(kThreads) paged_step_kernel(const StepArgs g) 
     int base_tok = __shfl_up_sync(0xFFFFFFFFu, inc_tok, 1), base_pages = __shfl_up_sync(0xFFFFFFFFu, inc_pages, 1);
     if (lane == 0) base_tok = base_pages = 0;
     __syncthreads();
-    int total_tok = 0, total_pages = 0;
-    for (int w = 0; w < 32; ++w) {
-        if (w == warp) base_tok = sat_add(base_tok, total_tok), base_pages = sat_add(base_pages, total_pages);
-        total_tok = sat_add(total_tok, warp_tok[w]), total_pages = sat_add(total_pages, warp_pages[w]);
+    // the warps' sums, scanned by every warp for itself
+    int wt = lane < kWarps ? warp_tok[lane] : 0, wp = lane < kWarps ? warp_pages[lane] : 0;
+#pragma unroll
+    for (int s = 1; s < kWarps; s <<= 1) {
+        const int a = __shfl_up_sync(0xFFFFFFFFu, wt, s), b = __shfl_up_sync(0xFFFFFFFFu, wp, s);
+        if (lane >= s) wt = sat_add(wt, a), wp = sat_add(wp, b);
     }
+    const int total_tok = __shfl_sync(0xFFFFFFFFu, wt, kWarps - 1), total_pages = __shfl_sync(0xFFFFFFFFu, wp, kWarps - 1);
+    const int prev_tok = __shfl_sync(0xFFFFFFFFu, wt, max(warp - 1, 0)), prev_pages = __shfl_sync(0xFFFFFFFFu, wp, max(warp - 1, 0));
+    if (warp > 0) base_tok = sat_add(base_tok, prev_tok), base_pages = sat_add(base_pages, prev_pages);
     for (int r = r0; r < r1; ++r) tok[r] = sat_add(tok[r], base_tok), pages[r] = sat_add(pages[r], base_pages);
     __syncthreads();
 
-    const int n_free = min(max(*g.n_free, 0), g.free_cap);
+    const int n_free = min(max(free_given, 0), g.free_cap);
     auto held_of = [&](int ctx) {
         return (int)min(((long long)ctx + (1 << g.page_shift) - 1) >> g.page_shift, (long long)g.W);
     };
@@ -169,7 +176,7 @@ extern "C" int deca_paged_step(const int32_t *ctx_lens, const int32_t *new_lens,
     if (int rc = current_device_info(&di)) return rc;
     const int64_t work = T > B ? T : B;
     int64_t grid = (work + kThreads - 1) / kThreads;
-    if (grid > di.sms) grid = di.sms;
+    if (grid > 4 * di.sms) grid = 4 * di.sms;
     static SmemLimitCache configured;
     const size_t smem = 3 * sizeof(int) * (size_t)B;
     if (int rc = ensure_dynamic_smem(paged_step_kernel, smem, configured)) return rc;

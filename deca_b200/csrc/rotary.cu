@@ -8,6 +8,7 @@
 // are computed once per token into shared memory and shared by all heads: for 48 heads of 128 that is
 // one sincospi per 96 elements.  What is left is a copy: every element is read once and written once.
 #include "common.cuh"
+#include "ptx.cuh"
 
 namespace deca {
 namespace {
@@ -29,6 +30,7 @@ struct RotArgs {
     long long n_slots;  // num_pages * page_size
     int page_shift;     // log2(page_size)
     int Hq, Hkv;        // Hkv = 0: no append
+    long long tokens;
     int D, rot;
     float amplitude;    // negative sign of the sine folded into `sine`
     float sine;
@@ -102,16 +104,15 @@ __device__ __forceinline__ void turn(Raw<V> &ra, Raw<V> &rb, const float2 *cs) {
     rb.template set<DT>(b);
 }
 
-constexpr int kUnits = 4;  // units of a thread whose loads are issued together
+constexpr int kUnits = 3;  // units of a thread whose loads are issued together
 
-// One CTA per token (or share of its heads, gridDim.y of them).  A unit is two parts of V elements of a head:
-// V whole pairs, or 2 V elements behind the rotated ones; a thread keeps its place within the head and
-// walks over the heads of q, then k, then v, so it needs one division.  Its first units are on their way
-// while the angles are computed.
+// A CTA takes every gridDim.x-th token (or a share of its heads, gridDim.y of them).  A unit is two parts of V
+// elements of a head: V whole pairs, or 2 V elements behind the rotated ones; a thread keeps its place within
+// the head and walks over the heads of q, then k, then v, so it needs one division.  A token's first units are on
+// their way while its angles are computed.
 template <int DT, int V, int LAYOUT>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotArgs g, const __grid_constant__ Turns turns) {
-    __shared__ float2 cs[kMaxPairs];
-    const long long tok = blockIdx.x;
+__global__ void __launch_bounds__(kThreads, 5) rotary_kernel(const RotArgs g, const __grid_constant__ Turns turns) {
+    __shared__ float2 angles[2][kMaxPairs];  // of two tokens in turn: one barrier per token
     const int per_head = g.D / (2 * V);
     const int at = blockIdx.y * blockDim.x + threadIdx.x;  // blockDim.x is a multiple of per_head
     const int u = at % per_head, step = (int)(blockDim.x * gridDim.y) / per_head;
@@ -119,64 +120,68 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotArgs g, const
     const bool split = LAYOUT == DECA_ROT_HALF && rotated;
     const int off_a = split ? u * V : u * 2 * V, off_b = split ? u * V + g.rot / 2 : u * 2 * V + V;
     const int heads = g.Hq + 2 * g.Hkv;
+    const unsigned long long my_turn = (int)threadIdx.x < g.rot / 2 ? turns.t[threadIdx.x] : 0ull;
+    float2 *cs = angles[0];
 
-    auto source = [&](int head) -> const char * {
-        if (head < g.Hq) return g.q + 2 * (tok * g.q_st + head * g.q_sh);
-        head -= g.Hq;
-        if (head < g.Hkv) return g.k + 2 * (tok * g.k_st + head * g.k_sh);
-        return g.v + 2 * (tok * g.v_st + (head - g.Hkv) * g.v_sh);
-    };
-    Raw<V> a[kUnits], b[kUnits];
-    int head = at / per_head;
-    auto load = [&]() {
+    for (long long tok = blockIdx.x; tok < g.tokens; tok += gridDim.x) {
+        auto source = [&](int head) -> const char * {
+            if (head < g.Hq) return g.q + 2 * (tok * g.q_st + head * g.q_sh);
+            head -= g.Hq;
+            if (head < g.Hkv) return g.k + 2 * (tok * g.k_st + head * g.k_sh);
+            return g.v + 2 * (tok * g.v_st + (head - g.Hkv) * g.v_sh);
+        };
+        Raw<V> a[kUnits], b[kUnits];
+        int head = at / per_head;
+        auto load = [&]() {
 #pragma unroll
-        for (int i = 0; i < kUnits; ++i)
-            if (head + i * step < heads) {
-                const char *src = source(head + i * step);
-                a[i].load(src + 2 * off_a);
-                b[i].load(src + 2 * off_b);
-            }
-    };
-    load();
-    long long row_k = -1, row_v = -1;  // element offsets of the token's cache rows, -1: none
-    if (g.Hkv > 0) {
-        const long long slot = g.slots[tok];
+            for (int i = 0; i < kUnits; ++i)
+                if (head + i * step < heads) {
+                    const char *src = source(head + i * step);
+                    a[i].load(src + 2 * off_a);
+                    b[i].load(src + 2 * off_b);
+                }
+        };
+        const long long pos = g.positions[tok];
+        const long long slot = g.Hkv > 0 ? g.slots[tok] : -1;
+        load();
+        for (int p = threadIdx.x; p < g.rot / 2; p += blockDim.x) {
+            const unsigned long long turn = p < (int)blockDim.x ? my_turn : turns.t[p];
+            const long long angle = (long long)((unsigned long long)pos * turn);  // 2^63 = half a turn
+            float s, c;
+            sincospif((float)angle * 1.0842021724855044e-19f, &s, &c);
+            cs[p] = make_float2(c * g.amplitude, s * g.sine);
+        }
+        long long row_k = -1, row_v = -1;  // element offsets of the token's cache rows, -1: none
         if (slot >= 0 && slot < g.n_slots) {
             const long long page = slot >> g.page_shift, row = slot & ((1ll << g.page_shift) - 1);
             row_k = page * g.kc_sp + row * g.kc_sr;
             row_v = page * g.vc_sp + row * g.vc_sr;
         }
-    }
-    const long long pos = g.positions[tok];
-    for (int p = threadIdx.x; p < g.rot / 2; p += blockDim.x) {
-        const long long angle = (long long)((unsigned long long)pos * turns.t[p]);  // 2^63 = half a turn
-        float s, c;
-        sincospif((float)angle * 1.0842021724855044e-19f, &s, &c);
-        cs[p] = make_float2(c * g.amplitude, s * g.sine);
-    }
-    __syncthreads();
-    while (true) {
+        __syncthreads();
+        while (true) {
 #pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-            int h = head + i * step;
-            if (h >= heads) break;
-            char *dst;
-            if (h < g.Hq) {
-                dst = g.qo + 2 * (tok * g.qo_st + h * g.qo_sh);
-            } else if ((h -= g.Hq) < g.Hkv) {
-                dst = row_k >= 0 ? g.kc + 2 * (row_k + h * g.kc_sh) : nullptr;
-            } else {
-                dst = row_v >= 0 ? g.vc + 2 * (row_v + (h - g.Hkv) * g.vc_sh) : nullptr;
+            for (int i = 0; i < kUnits; ++i) {
+                int h = head + i * step;
+                if (h >= heads) break;
+                char *dst;
+                if (h < g.Hq) {
+                    dst = g.qo + 2 * (tok * g.qo_st + h * g.qo_sh);
+                } else if ((h -= g.Hq) < g.Hkv) {
+                    dst = row_k >= 0 ? g.kc + 2 * (row_k + h * g.kc_sh) : nullptr;
+                } else {
+                    dst = row_v >= 0 ? g.vc + 2 * (row_v + (h - g.Hkv) * g.vc_sh) : nullptr;
+                }
+                if (rotated && head + i * step < g.Hq + g.Hkv) turn<DT, V, LAYOUT>(a[i], b[i], cs + u * V);
+                if (dst) {
+                    a[i].store(dst + 2 * off_a);
+                    b[i].store(dst + 2 * off_b);
+                }
             }
-            if (rotated && head + i * step < g.Hq + g.Hkv) turn<DT, V, LAYOUT>(a[i], b[i], cs + u * V);
-            if (dst) {
-                a[i].store(dst + 2 * off_a);
-                b[i].store(dst + 2 * off_b);
-            }
+            head += kUnits * step;
+            if (head >= heads) break;
+            load();
         }
-        head += kUnits * step;
-        if (head >= heads) return;
-        load();
+        cs = cs == angles[0] ? angles[1] : angles[0];
     }
 }
 
@@ -217,14 +222,18 @@ int launch_rotary(int dtype, RotArgs &g, const deca_rotation *r, long long token
     const int heads = g.Hq + 2 * g.Hkv;
     // Threads: as few groups of a head's units as cover the heads in whole rounds, about `want` units each
     const int most = kThreads / per_head;  // heads that a CTA of full size takes at once
-    const int want = tokens < 296 ? 1 : 3;
+    const int want = tokens < 296 ? 1 : kUnits;
     int at_once = (heads + want - 1) / want;
     if (at_once * per_head < 64) at_once = (63 + per_head) / per_head;  // the angles want two warps
     if (at_once > most) at_once = most;
     // few tokens: the heads of a token are shared by several CTAs
     int split = 1;
     while (tokens * split < 296 && split * at_once < heads && split < 64) split *= 2;
-    const dim3 grid((unsigned)tokens, (unsigned)split);
+    g.tokens = tokens;
+    DeviceInfo di;
+    if (int rc = current_device_info(&di)) return rc;
+    const int resident = di.sms * (40 / ((at_once * per_head + 31) / 32));  // CTAs that run at once: 40 warps an SM
+    const dim3 grid((unsigned)(tokens < resident ? tokens : resident), (unsigned)split);
     const unsigned threads = (unsigned)(at_once * per_head);
     if (dtype == DECA_F16)
         vec ? launch_layout<DECA_F16, 8>(g, t, r->layout, grid, threads, st) : launch_layout<DECA_F16, 1>(g, t, r->layout, grid, threads, st);
