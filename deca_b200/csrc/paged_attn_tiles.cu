@@ -52,8 +52,11 @@ struct RingPos {
     uint32_t par;
 };
 
-// Exponentials of 32 scores against the maximum's term: packed to 16 bits, summed in fp32.  A masked score is -inf;
-// the polynomial share would make 2^-126 of it, hence the selection there.
+// What the polynomial share makes of -inf: its constant term with 2^-126 put into the exponent (0x3F7FFB43 less
+// 126 << 23).  Taken off every polynomial value, it leaves a masked score exactly zero.
+constexpr float kPolyLeast = 0x1.ffed0cp-127f;
+
+// Exponentials of 32 scores against the maximum's term: packed to 16 bits, summed in fp32.  A masked score is -inf.
 template <int DT, int EVERY>
 __device__ __forceinline__ void exp_chunk32(const uint32_t (&v)[32], uint64_t sl2x2, uint64_t nmsx2, const FaPolyConst &pc,
                                             uint64_t (&sum2)[2], uint32_t *pk) {
@@ -63,8 +66,7 @@ __device__ __forceinline__ void exp_chunk32(const uint32_t (&v)[32], uint64_t sl
         float p0, p1;
         if (EVERY > 0 && i % (EVERY > 0 ? EVERY : 1) == (EVERY > 0 ? EVERY : 1) - 1) {
             fa_exp2_poly_pair(s0, s1, pc, p0, p1);
-            if (v[2 * i] == 0xFF800000u) p0 = 0.f;
-            if (v[2 * i + 1] == 0xFF800000u) p1 = 0.f;
+            f32x2_unpack(f32x2_add(f32x2_pack(p0, p1), f32x2_pack(-kPolyLeast, -kPolyLeast)), p0, p1);
         } else {
             float x0, x1;
             f32x2_unpack(f32x2_fma(f32x2_pack(s0, s1), sl2x2, nmsx2), x0, x1);
@@ -121,9 +123,10 @@ __device__ __forceinline__ void mask_tile(uint32_t tS, int visible) {
 
 // One key tile of the online softmax for this thread's row.  A row sees a prefix of the keys, so one that
 // sees nothing of a segment's first 32 keys sees nothing of it: m stays -inf, l and P zero.
-// There is one copy of the exponentials' code for both passes, and masked tiles are masked in place before it: the
-// warps' roles share the instruction cache, and what falls out of it costs an item microseconds when it ends
-// (with a copy for each case 4 us from the last product of an item to the first score of the next).
+// There is one copy of the exponentials' straight-line code: masked tiles are masked in place before it, and the
+// rare second pass is a loop.  The warps' roles share the instruction cache, and what falls out of it costs an
+// item microseconds when it ends (with a copy for each case 4 us from the last product of an item to the first
+// score of the next).
 template <int DT, int D>
 __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, float sl2, bool first, float &m, float &l) {
     if (first) {
@@ -132,45 +135,65 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, float sl2
         tmem_ld_wait();
         m = max32(v);
     }
-    uint32_t pk[kBc / 2];
-    float sum;
-#pragma unroll 1
-    for (bool again = false;; again = true) {
+    {
         // held in registers until the vote: storing P overwrites the scores that a second pass would need
-        sum = exp_row<DT, kFaPolyEveryFor<D>>(tS, sl2, m == -INFINITY ? 0.f : m * sl2, pk);
-        if (again || !__any_sync(0xFFFFFFFFu, !(sum <= kFaSumLimit))) break;
-        float top = m;
-#pragma unroll 1
-        for (int c = 0; c < kBc / 32; ++c) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(tS + c * 32, v);
-            tmem_ld_wait();
-            top = fmaxf(top, max32(v));
-        }
-        const float alpha = m == -INFINITY ? 0.f : ex2_approx((m - top) * sl2);
-        l *= alpha;
-        m = top;
-        if (!first) {
-            // the product of the previous tile is complete: it was issued before this tile's scores
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(tO + c * 32, v);
-                tmem_ld_wait();
+        uint32_t pk[kBc / 2];
+        const float sum = exp_row<DT, kFaPolyEveryFor<D>>(tS, sl2, m == -INFINITY ? 0.f : m * sl2, pk);
+        if (!__any_sync(0xFFFFFFFFu, !(sum <= kFaSumLimit))) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
-                tmem_st_32x32b_x32(tO + c * 32, v);
+            for (int h = 0; h < kBc / 64; ++h) {
+                uint32_t part[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) part[i] = pk[h * 32 + i];
+                tmem_st_32x32b_x32(tS + h * 32, part);
             }
             tmem_st_wait();
+            l += sum;
+            return;
         }
     }
-    l += sum;
+    float top = m;
+#pragma unroll 1
+    for (int c = 0; c < kBc / 32; ++c) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tS + c * 32, v);
+        tmem_ld_wait();
+        top = fmaxf(top, max32(v));
+    }
+    const float alpha = m == -INFINITY ? 0.f : ex2_approx((m - top) * sl2);
+    l *= alpha;
+    m = top;
+    if (!first) {
+        // the product of the previous tile is complete: it was issued before this tile's scores
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(tO + c * 32, v);
+            tmem_ld_wait();
 #pragma unroll
-    for (int h = 0; h < kBc / 64; ++h) {
-        uint32_t part[32];
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+            tmem_st_32x32b_x32(tO + c * 32, v);
+        }
+    }
+    // P of scores 64 c .. goes over columns that have been read
+    const float ms = m == -INFINITY ? 0.f : m * sl2;
+#pragma unroll 1
+    for (int c = 0; c < kBc / 64; ++c) {
+        uint32_t pk[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) part[i] = pk[h * 32 + i];
-        tmem_st_32x32b_x32(tS + h * 32, part);
+        for (int h = 0; h < 2; ++h) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(tS + c * 64 + h * 32, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p0 = ex2_approx(fmaf(__uint_as_float(v[2 * i]), sl2, -ms));
+                const float p1 = ex2_approx(fmaf(__uint_as_float(v[2 * i + 1]), sl2, -ms));
+                l += p0 + p1;
+                pk[h * 16 + i] = Pack16<DT>::pack(p0, p1);
+            }
+        }
+        tmem_st_32x32b_x32(tS + c * 32, pk);
     }
     tmem_st_wait();
 }
