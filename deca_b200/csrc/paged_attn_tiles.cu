@@ -240,9 +240,16 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     WorkPos w;
     allow_next_kernel();
     WorkShare *share = reinterpret_cast<WorkShare *>(smem + L::share);
-    // the ring is free for the costs
-    if (!find_work<TL>(g, w, share, reinterpret_cast<unsigned long long *>(smem + L::kv), (int)(kStages * L::kKVBytes / 8))) return;
-    ReqView v = request_view(g, w.req);
+    ReqView v;
+    int part_no = 0, n_parts = 0;  // > 0: this CTA has this one part of an item
+    const int found = find_part<TL>(g, w, v, part_no, n_parts);
+    if (found < 0) return;
+    if (found == 0) {
+        n_parts = 0;
+        // the ring is free for the costs
+        if (!find_work<TL>(g, w, share, reinterpret_cast<unsigned long long *>(smem + L::kv), (int)(kStages * L::kKVBytes / 8))) return;
+        v = request_view(g, w.req);
+    }
 
     // rows of the Q tiles that no token reaches stay zero
     for (int i = threadIdx.x; i < 2 * (D / 64) * (kBr - used) * 8; i += kThreads) {
@@ -294,7 +301,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     };
     auto next = [&](int n) {
         w.left -= n;
-        return w.left > 0 && next_item<TL>(g, w, v);
+        return w.left > 0 && n_parts == 0 && next_item<TL>(g, w, v);
     };
     // keys that the item reads, and the last one that all of its rows see
     auto item_keys = [&](int &kend, int &common) {
@@ -648,7 +655,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 part[(size_t)TL::ROWS * D + TL::ROWS + grp * kBr + r] = l;
                 if (starts && threadIdx.x == 64) {
                     PartialItem it;
-                    it.last = cta_of(share, share->end + (steps - n) - 1);
+                    it.last = n_parts > 0 ? (int)blockIdx.x + n_parts - 1 : cta_of(share, share->end + (steps - n) - 1);
                     it.head = w.head, it.tile = w.tile, it.q0 = v.q0, it.n = v.n;
                     g.meta[blockIdx.x] = it;
                 }
