@@ -398,7 +398,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 for (int j = -1; j < n && ok; ++j) {
                     const uint64_t kdesc = kDescK | (uint64_t)(((sKV + kp.slot * L::kKVBytes) & 0x3FFFFu) >> 4);
                     const uint64_t vdesc = kDescV | (uint64_t)(((sKV + vp.slot * L::kKVBytes) & 0x3FFFFu) >> 4);
-#pragma unroll 1
+#pragma unroll
                     for (int grp = 0; grp < 2; ++grp) {
                         const uint32_t s_tmem = tS(grp), o_tmem = tO(grp);
                         if (j >= 0) {
