@@ -3,6 +3,8 @@
     python -m deca_b200.run_case --op softmax --dtype fp16 --shape 16384 4096 --iters 5
     python -m deca_b200.run_case --op gemm --shape 4096 4096 4096
     python -m deca_b200.run_case --op attention --shape 4 16 4096 128 [--causal]
+    python -m deca_b200.run_case --op add_rmsnorm --dtype bf16 --shape 16384 8192 [--out e4m3 --group 128]
+    python -m deca_b200.run_case --op paged_attention --dtype bf16 --shape B H_q H_kv D page_size max_q max_kv
 
 Prints the median CUDA-event time and the throughput in the operator's unit.
 """
@@ -11,15 +13,18 @@ import argparse
 
 import torch
 
-from .operators import GEMMTC, FlashAttention, RMSNorm, Softmax
+from .operators import GEMMTC, AddRMSNorm, FlashAttention, PagedAttention, RMSNorm, Softmax
 
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("--op", choices=["softmax", "rmsnorm", "gemm", "attention"], required=True)
+    ap.add_argument("--op", choices=["softmax", "rmsnorm", "gemm", "attention", "add_rmsnorm", "paged_attention"],
+                    required=True)
     ap.add_argument("--dtype", default="fp16")
     ap.add_argument("--shape", nargs="+", type=int, required=True)
     ap.add_argument("--causal", action="store_true")
+    ap.add_argument("--out", choices=["same", "e4m3"], default="same", help="add_rmsnorm: type of the output")
+    ap.add_argument("--group", type=int, default=0, help="add_rmsnorm: columns per scale (0: one scale a row)")
     ap.add_argument("--iters", type=int, default=5)
     ap.add_argument("--config", default="", help="key=value,... overrides of the default config")
     args = ap.parse_args()
@@ -30,6 +35,10 @@ def main():
         op = Softmax(M, N, dt) if args.op == "softmax" else RMSNorm(M, N, dt)
     elif args.op == "gemm":
         op = GEMMTC(*args.shape, dtype=dt)
+    elif args.op == "add_rmsnorm":
+        op = AddRMSNorm(*args.shape, dtype=dt, out=args.out, group=args.group)
+    elif args.op == "paged_attention":
+        op = PagedAttention(*args.shape, dtype=dt)
     else:
         B, H, S, D = args.shape
         op = FlashAttention(B, H, S, S, D, causal=args.causal)

@@ -159,6 +159,40 @@ def test_graph_and_repeatability():
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
 
+def test_offsets_past_31_bits():
+    from deca_b200.operators import AddRMSNorm
+
+    M, N = 2**31 // 8192 + 3, 8192
+    x, res = (torch.zeros(M, N, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    tail = inputs(3, N, "bfloat16")
+    x[-3:], res[-3:] = tail[0], tail[1]
+    y, h = AddRMSNorm(M, N, "bfloat16")(x, res, tail[2], res_out=res)
+    want_h, want_y = exact(*tail, 1e-6)
+    check(h[-3:], want_h, "bfloat16", 1e-7)
+    check(y[-3:], want_y, "bfloat16", 1e-5)
+    assert (y[-4] == 0).all()
+
+
+def test_harness_and_command_line():
+    """The tuning harness verifies and times the operator, and run_case prints its rate."""
+    import subprocess
+    import sys
+
+    from deca_b200.arch.B200 import B200
+    from deca_b200.operators import AddRMSNorm, PagedAttention
+    from deca_b200.RuntimeMod import RuntimeMod
+
+    for op in (AddRMSNorm(300, 1000, "bf16"), AddRMSNorm(300, 1000, "bf16", out="e4m3", group=128), PagedAttention(2, 8, 2, 64, 16, 40, 300),
+               PagedAttention(2, 8, 2, 128, 16, 1, 300, "bf16")):
+        rt = RuntimeMod(op, B200(), False, op.default_config())
+        rt.build()
+        rt.time_evaluator()
+        assert rt.throughput > 0 and op.name in rt.record
+    for args in ("--op add_rmsnorm --dtype bf16 --shape 64 4096 --out e4m3", "--op paged_attention --shape 2 8 2 128 16 1 500"):
+        res = subprocess.run([sys.executable, "-m", "deca_b200.run_case", *args.split(), "--iters", "2"], capture_output=True, text=True)
+        assert res.returncode == 0 and " ms, " in res.stdout, res.stderr[-500:]
+
+
 def test_empty_batch():
     from deca_b200.operators import AddRMSNorm
 

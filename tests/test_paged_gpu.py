@@ -142,11 +142,31 @@ def test_long_context_is_split_and_joined(dtype, max_q):
         assert torch.equal(a, b)
 
 
-def test_many_requests():
+@pytest.mark.parametrize("max_q,max_kv", [(1, 90), (1, 100000), (1000, 90)])
+def test_many_requests(max_q, max_kv):
+    """More (request, key head) pairs than CTAs: taken whole, cut anywhere, and on tensor-core tiles."""
     g = torch.Generator().manual_seed(9)
-    kv = torch.randint(1, 90, (700,), generator=g).tolist()
+    kv = torch.randint(0, 90, (700,), generator=g).tolist()
     data = make_paged(kv, [1] * 700, 4, 2, 64, 16, torch.float16)
-    check(run(*data, 16), *data)
+    check(run(*data, 16, max_q=max_q, max_kv=max_kv), *data)
+
+
+@pytest.mark.parametrize("new", [1, 3])
+def test_long_ragged_batch_is_cut_between_requests(new):
+    """Long contexts on more pairs than CTAs: a CTA's steps start and end inside items."""
+    g = torch.Generator().manual_seed(3)
+    kv = torch.randint(3, 2500, (40,), generator=g).tolist()
+    data = make_paged(kv, [new] * 40, 8, 8, 128, 32, torch.bfloat16)
+    a, b = (run(*data, 32, max_kv=20000) for _ in range(2))
+    check(a, *data)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("H_q,H_kv,new", [(128, 1, 2), (200, 2, 3), (24, 1, 1), (40, 2, 70), (31, 1, 33)])
+def test_wide_and_odd_groups(H_q, H_kv, new):
+    data = make_paged([1500, 77], [new, 1], H_q, H_kv, 64, 64, torch.float16)
+    check(run(*data, 64), *data)
+    check(run(*data, 64, max_q=1, max_kv=100), *data)
 
 
 @pytest.mark.parametrize("new,max_q", [([3, 40], None), ([3, 40], 1), ([1, 1], None)])
@@ -173,7 +193,7 @@ def test_scales(scale, max_q):
     check(run(*data, 16, max_q=max_q, scale=scale), *data, scale=scale)
 
 
-@pytest.mark.parametrize("max_q", [1, 1000])
+@pytest.mark.parametrize("max_q", [1, 12, 1000])
 @pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
 def test_what_a_row_does_not_see_never_reaches_it(value, max_q):
     """A key of the chunk itself that is not finite: tokens before it are untouched, tokens from it on are
@@ -266,6 +286,53 @@ def test_graphs_streams_and_two_calls_at_once():
         torch.cuda.synchronize()
         for o, w in zip(outs, want):
             assert torch.equal(o, w)
+
+
+def test_one_operator_in_two_threads():
+    """Two host threads call one operator object on streams of their own."""
+    import threading
+
+    from deca_b200.operators import PagedAttention
+
+    sets = [make_paged([9000, 500], [1, 1], 8, 2, 128, 64, torch.bfloat16, seed=s) for s in (5, 6)]
+    op = PagedAttention(2, 8, 2, 128, 64, 1, 9000, "bfloat16")
+    args = [(q, kc, vc, t, i32(cu), i32(kv)) for q, kc, vc, t, cu, kv in sets]
+    want = [op(*a) for a in args]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                got = op(*args[i])
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(got, want[i]):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.parametrize("max_q", [1, 1000])
+def test_offsets_past_31_bits(max_q):
+    """Pages whose first element lies behind 2^31 of a cache."""
+    from deca_b200.operators import RotaryAppend
+
+    q, kc, vc, table, cu, kv = make_paged([300, 40], [5, 7], 8, 8, 128, 256, torch.float16, fill=0.0)
+    pages = 2**31 // (256 * 8 * 128) + 6  # of 262144 elements
+    far_k, far_v = (torch.empty(pages, 256, 8, 128, dtype=q.dtype, device="cuda") for _ in range(2))
+    shift = pages - kc.shape[0]
+    far_k[shift:], far_v[shift:] = kc, vc
+    got = run(q, far_k, far_v, table + shift, cu, kv, 256, max_q=max_q)
+    check(got, q, kc, vc, table, cu, kv)
+    slots = torch.tensor([(pages - 1) * 256 + 3], device="cuda")
+    one = torch.ones(1, 8, 128, dtype=q.dtype, device="cuda")
+    RotaryAppend(8, 8, 128, 256)(one, one, 2 * one, i32([0]), slots, far_k, far_v)
+    assert (far_k[-1, 3] == 1).all() and (far_v[-1, 3] == 2).all() and (far_k[-1, 4] == kc[-1, 4]).all()
 
 
 def test_attention_refusals():
