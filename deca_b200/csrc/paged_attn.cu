@@ -38,9 +38,24 @@ bool use_cuts(const deca_paged_attn_args &a, int sms) {
     const double us = pairs * a.max_kv * a.D * 2.0 / 6.5e6, rounds = std::ceil(pairs / ctas);
     return pairs <= ctas ? us > 60 : us * (rounds * ctas / pairs - 1.0) > 15;
 }
-// ... and tensor maps want strides that advance
-bool strides_ok(const PagedArgs &g) {
-    return g.q_st > 0 && g.q_sh > 0 && g.k_sp > 0 && g.k_sr > 0 && g.k_sh > 0 && g.v_sp > 0 && g.v_sr > 0 && g.v_sh > 0;
+// Tensor maps want strides that advance.  A dimension of one element may have any; a head stride of zero (one key head
+// expanded to several) becomes a dimension of one element.
+bool normalise(int64_t &stride, int64_t extent, int64_t any) {
+    if (extent <= 1) stride = any;
+    return stride > 0;
+}
+bool cache_strides(const deca_paged_attn_args &a, const deca_cache &c, long long &sp, long long &sr, long long &sh, int &heads) {
+    int64_t p = c.page_stride, r = c.row_stride, h = c.head_stride;
+    heads = a.H_kv > 1 && h == 0 ? 0 : 1;
+    const bool ok = normalise(p, a.num_pages, a.D) && normalise(r, a.page_size, a.D) && normalise(h, heads ? a.H_kv : 1, a.D);
+    sp = p, sr = r, sh = h;
+    return ok;
+}
+bool query_strides(const deca_paged_attn_args &a, long long &st, long long &sh) {
+    int64_t t = a.Q.token_stride, h = a.Q.head_stride;
+    const bool ok = normalise(t, a.T, a.D) && normalise(h, a.H_q, a.D);
+    st = t, sh = h;
+    return ok;
 }
 
 }  // namespace
@@ -62,6 +77,9 @@ extern "C" int deca_paged_attn_check(const deca_paged_attn_args *a) {
     if (!(a->scale == a->scale) || a->scale - a->scale != 0.f) return DECA_ERR_CONFIG;  // NaN or infinite
     if (!a->Q.data || !a->O.data || !a->K.data || !a->V.data || !a->block_table || !a->cu_q || !a->kv_lens) return DECA_ERR_NULL;
     if (!tokens_ok(a->Q) || !tokens_ok(a->O) || !cache_ok(a->K) || !cache_ok(a->V)) return DECA_ERR_ALIGN;
+    long long sp, sr, sh;
+    int heads;
+    if (!cache_strides(*a, a->K, sp, sr, sh, heads) || !cache_strides(*a, a->V, sp, sr, sh, heads)) return DECA_ERR_ALIGN;
     if (!aligned_to(a->block_table, 4) || !aligned_to(a->cu_q, 4) || !aligned_to(a->kv_lens, 4)) return DECA_ERR_ALIGN;
     return DECA_OK;
 }
@@ -89,8 +107,9 @@ extern "C" int deca_paged_attn(const deca_paged_attn_args *a, void *stream) {
     PagedArgs g = {};
     g.q = static_cast<const char *>(a->Q.data), g.q_st = a->Q.token_stride, g.q_sh = a->Q.head_stride;
     g.o = static_cast<char *>(a->O.data), g.o_st = a->O.token_stride, g.o_sh = a->O.head_stride;
-    g.k = static_cast<const char *>(a->K.data), g.k_sp = a->K.page_stride, g.k_sr = a->K.row_stride, g.k_sh = a->K.head_stride;
-    g.v = static_cast<const char *>(a->V.data), g.v_sp = a->V.page_stride, g.v_sr = a->V.row_stride, g.v_sh = a->V.head_stride;
+    g.k = static_cast<const char *>(a->K.data), g.v = static_cast<const char *>(a->V.data);
+    cache_strides(*a, a->K, g.k_sp, g.k_sr, g.k_sh, g.k_heads);
+    cache_strides(*a, a->V, g.v_sp, g.v_sr, g.v_sh, g.v_heads);
     g.table = a->block_table, g.table_stride = a->table_stride, g.W = a->table_width;
     g.cu = a->cu_q, g.kv_lens = a->kv_lens;
     g.T = a->T, g.num_pages = a->num_pages, g.B = a->B, g.Hkv = a->H_kv, g.group = a->H_q / a->H_kv;
@@ -99,7 +118,7 @@ extern "C" int deca_paged_attn(const deca_paged_attn_args *a, void *stream) {
     g.sl2 = a->scale * kLog2e;
     g.status = device_status_ptr();
     if (!g.status) return (int)cudaErrorUnknown;
-    if (use_tiles(*a) && strides_ok(g)) {
+    if (use_tiles(*a) && query_strides(*a, g.q_st, g.q_sh)) {
         g.min_steps = 2;
         g.max_parts = 1 << 20;
         return paged_tiles_launch(*a, g, di.sms, static_cast<cudaStream_t>(stream));

@@ -11,6 +11,7 @@
 #pragma once
 
 #include "ptx.cuh"
+#include "tmap.cuh"
 
 namespace deca {
 
@@ -24,6 +25,7 @@ struct PagedArgs {
     long long T, num_pages;
     int B, W, Hkv, group;  // group: query heads per key head
     int tile_tokens;       // TokenTiles: whole tokens in 128 rows
+    int k_heads, v_heads;  // 0 where all key heads lie at the same place (a head stride of zero), else 1
     int page_shift;
     int causal;
     float sl2;  // scale * log2 e
@@ -367,6 +369,19 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
         join_row<TL::ROWS, D, 4>(part, it.last - c0 + 1, row, lane, acc, sum);
         store_joined<DT, D>(g.o + 2 * (((long long)it.q0 + tok) * g.o_st + (long long)(it.head * g.group + j) * g.o_sh), lane, acc, sum);
     }
+}
+
+// Tensor maps of the caches, (d, row of the page, key head, page), with boxes of 64 columns and the rows of a page
+// or `keys`, whichever is less.
+inline int make_cache_maps(CUtensorMap *tmK, CUtensorMap *tmV, int dtype, int D, int keys, const PagedArgs &g) {
+    const uint64_t page = 1ull << g.page_shift;
+    const uint32_t box[4] = {64, (uint32_t)(page < (uint64_t)keys ? page : keys), 1, 1};
+    const uint64_t kd[4] = {(uint64_t)D, page, g.k_heads ? (uint64_t)g.Hkv : 1, (uint64_t)g.num_pages};
+    const uint64_t vd[4] = {(uint64_t)D, page, g.v_heads ? (uint64_t)g.Hkv : 1, (uint64_t)g.num_pages};
+    const uint64_t ks[3] = {(uint64_t)g.k_sr * 2, (uint64_t)g.k_sh * 2, (uint64_t)g.k_sp * 2};
+    const uint64_t vs[3] = {(uint64_t)g.v_sr * 2, (uint64_t)g.v_sh * 2, (uint64_t)g.v_sp * 2};
+    if (int rc = make_tmap_16bit(tmK, dtype, g.k, 4, kd, ks, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+    return make_tmap_16bit(tmV, dtype, g.v, 4, vd, vs, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Lets the next kernel of the stream be scheduled while this one drains (it waits for the results itself).

@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(32 * NW, CPS) paged_rows_kernel(const PagedArg
                 return i < n_tiles && key < kend ? table[key >> g.page_shift] : -1;
             };
             int pages = page_of(lane), pages_next = page_of(32 + lane);  // of 32 tiles each
-            const char *kh = g.k + 2 * ((long long)w.head * g.k_sh), *vh = g.v + 2 * ((long long)w.head * g.v_sh);
+            const char *kh = g.k + 2 * ((long long)(w.head * g.k_heads) * g.k_sh), *vh = g.v + 2 * ((long long)(w.head * g.v_heads) * g.v_sh);
             auto issue = [&](int i, int slot) {
                 if (i < n_tiles) {
                     if ((i & 31) == 0 && i > 0) {

@@ -361,7 +361,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     if (lane == 0) mbar_arrive_expect_tx(kv_full(rp.slot), (uint32_t)(live * rows * D * 2));
                     __syncwarp();
                     if (page >= 0)
-                        tma_load_4d(dst + rp.slot * L::kKVBytes, kv ? &tmV : &tmK, blk * 64, row, w.head, page, kv_full(rp.slot));
+                        tma_load_4d(dst + rp.slot * L::kKVBytes, kv ? &tmV : &tmK, blk * 64, row,
+                                    w.head * (kv ? g.v_heads : g.k_heads), page, kv_full(rp.slot));
                     advance(rp, 1);
                 }
                 page = page_next;
@@ -693,13 +694,7 @@ int launch_tiles(const PagedArgs &g, const deca_paged_attn_args &a, int sms, cud
         const uint32_t box[4] = {64, (uint32_t)group, 1, (uint32_t)(128 / g.group)};
         if (int rc = make_tmap_16bit(&tmQ, DT, g.q, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
     }
-    const uint64_t page = 1ull << g.page_shift;
-    const uint64_t dims[4] = {(uint64_t)D, page, (uint64_t)g.Hkv, (uint64_t)g.num_pages};
-    const uint32_t box[4] = {64, (uint32_t)(page < kBc ? page : kBc), 1, 1};
-    const uint64_t ks[3] = {(uint64_t)g.k_sr * 2, (uint64_t)g.k_sh * 2, (uint64_t)g.k_sp * 2};
-    const uint64_t vs[3] = {(uint64_t)g.v_sr * 2, (uint64_t)g.v_sh * 2, (uint64_t)g.v_sp * 2};
-    if (int rc = make_tmap_16bit(&tmK, DT, g.k, 4, dims, ks, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
-    if (int rc = make_tmap_16bit(&tmV, DT, g.v, 4, dims, vs, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+    if (int rc = make_cache_maps(&tmK, &tmV, DT, D, kBc, g)) return rc;
     static SmemLimitCache configured;
     if (int rc = ensure_dynamic_smem(paged_tiles_kernel<DT, D>, Layout<D>::smem, configured)) return rc;
     paged_tiles_kernel<DT, D><<<(unsigned)sms, kThreads, Layout<D>::smem, st>>>(tmQ, tmK, tmV, g);

@@ -232,6 +232,20 @@ def test_strides_and_untouched_rows(max_q):
 
 
 @pytest.mark.parametrize("max_q", [1, 1000])
+def test_one_key_head_expanded(max_q):
+    """A cache of one key head seen as four (a head stride of zero) is that head four times; query rows that do not
+    advance are read as they lie; a cache whose rows do not advance is refused."""
+    q, kc, vc, table, cu, kv = make_paged([300, 70], [40, 1], 8, 1, 64, 32, torch.bfloat16, fill=0.0)
+    wide_k, wide_v = kc.expand(-1, -1, 4, -1), vc.expand(-1, -1, 4, -1)
+    got = run(q, wide_k, wide_v, table, cu, kv, 32, max_q=max_q)
+    check(got, q, wide_k, wide_v, table, cu, kv)
+    same = q[:1].expand(41, 8, 64)
+    check(run(same, kc, vc, table, cu, kv, 32, max_q=max_q), same, kc, vc, table, cu, kv)
+    with pytest.raises(RuntimeError, match="aligned"):
+        run(q, kc[:, :1].expand(-1, 32, -1, -1), vc, table, cu, kv, 32, max_q=max_q)
+
+
+@pytest.mark.parametrize("max_q", [1, 1000])
 def test_senseless_lengths_and_tables(max_q):
     """Lengths are clipped to what Q and the table hold and entries that name no page read as zeros."""
     q, kc, vc, table, cu, kv = make_paged([60, 40], [4, 20], 4, 2, 64, 16, torch.float16, fill=0.0)
