@@ -12,6 +12,7 @@
 // The running maximum moves only when a score exceeds it by 2^8 (it then rescales the numerators);
 // otherwise the exponentials are taken against the old one, as in the dense attention kernels.
 #include <atomic>
+#include <chrono>
 #include <random>
 
 #include "paged_attn.cuh"
@@ -449,8 +450,14 @@ size_t flag_bytes(int ctas) { return ((size_t)ctas * 2 * sizeof(unsigned long lo
 // A number that no other launch of any process carries, but for one chance in 2^64 or so.
 unsigned long long launch_tag() {
     static std::atomic<unsigned long long> next{[] {
-        std::random_device rd;
-        return ((unsigned long long)rd() << 32) ^ (unsigned long long)rd() ^ 0x9E3779B97F4A7C15ull;
+        unsigned long long seed = (unsigned long long)std::chrono::system_clock::now().time_since_epoch().count();
+        try {
+            std::random_device rd;
+            seed ^= ((unsigned long long)rd() << 32) ^ (unsigned long long)rd();
+        } catch (...) {  // no source of randomness: the clock and where the library lies have to do
+            seed ^= (unsigned long long)reinterpret_cast<uintptr_t>(&flag_bytes) << 20;
+        }
+        return seed;
     }()};
     unsigned long long t = next.fetch_add(0x9E3779B97F4A7C15ull);  // odd: runs through all 2^64 values
     return t ? t : next.fetch_add(0x9E3779B97F4A7C15ull);          // 0 is a cleared flag

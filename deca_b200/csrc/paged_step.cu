@@ -160,9 +160,30 @@ extern "C" int deca_paged_step(const int32_t *ctx_lens, const int32_t *new_lens,
     if (table_stride < table_width) return DECA_ERR_SHAPE;
     if (!ctx_lens || !new_lens || !block_table || !n_free || !cu_q || !kv_lens || !n_free_out || !short_out) return DECA_ERR_NULL;
     if ((free_capacity > 0 && !free_pages) || (T > 0 && (!positions || !slots))) return DECA_ERR_NULL;
-    // every CTA reads the lengths while others write
-    if (kv_lens == ctx_lens || kv_lens == new_lens || cu_q == ctx_lens || cu_q == new_lens || n_free_out == n_free)
-        return DECA_ERR_UNSUPPORTED;
+    // every CTA reads the inputs while others write
+    struct Span {
+        const void *at;
+        int64_t bytes;
+    };
+    const Span in[] = {{ctx_lens, 4ll * B}, {new_lens, 4ll * B}, {free_pages, 4ll * free_capacity}, {n_free, 4},
+                       {block_table, 4 * ((B - 1) * table_stride + table_width)}};
+    const Span out[] = {{cu_q, 4ll * (B + 1)}, {kv_lens, 4ll * B}, {positions, 4 * T}, {slots, 8 * T}, {n_free_out, 4}, {short_out, 4}};
+    auto meet = [](const Span &a, const Span &b) {
+        const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+        return a.bytes > 0 && b.bytes > 0 && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+    };
+    for (int i = 0; i < 6; ++i) {
+        for (const Span &s : in)
+            if (meet(out[i], s)) return DECA_ERR_UNSUPPORTED;
+        for (int j = 0; j < i; ++j)
+            if (meet(out[i], out[j])) return DECA_ERR_UNSUPPORTED;
+    }
+    for (int i = 0; i < 4; ++i)
+        if (meet(in[4], in[i])) return DECA_ERR_UNSUPPORTED;  // the table is written too
+    for (const Span &sp : in)
+        if (!aligned_to(sp.at, 4)) return DECA_ERR_ALIGN;
+    for (const Span &sp : out)
+        if (!aligned_to(sp.at, sp.at == slots ? 8 : 4)) return DECA_ERR_ALIGN;
     StepArgs g;
     g.ctx = ctx_lens, g.add = new_lens, g.table = block_table, g.table_stride = table_stride;
     g.free_pages = free_pages, g.n_free = n_free;

@@ -325,7 +325,8 @@ int deca_rotary_append(int dtype, const deca_tokens *Q, const deca_tokens *K, co
  *   positions[T], slots[T]  of token t of the step: its place in its request, and
  *                 page * page_size + row of the cache (-1 where it has no page).  Entries behind the last
  *                 token get position 0 and slot -1; tokens beyond T are not written.
- * Negative lengths count as 0.  Outputs must not overlap the inputs.  B <= 8192, page_size a power of two.
+ * Negative lengths count as 0.  Outputs must not overlap the inputs or each other (DECA_ERR_UNSUPPORTED).
+ * B <= 8192, page_size a power of two.
  * ------------------------------------------------------------------------------------- */
 int deca_paged_step(const int32_t *ctx_lens, const int32_t *new_lens, int B, int32_t *block_table,
                     int64_t table_stride, int table_width, const int32_t *free_pages, int free_capacity,
@@ -342,7 +343,8 @@ int deca_paged_step(const int32_t *ctx_lens, const int32_t *new_lens, int B, int
  * Lengths are read on the device and clipped to what T and the table hold; a table entry that names no
  * page reads as zeros.  What a row cannot see never reaches it, whatever the cache holds there.
  * max_q / max_kv: upper bounds of a request's new tokens and cached length as the caller knows them;
- * they choose the schedule (any values give right results).
+ * they choose the schedule (any values give right results).  O may be Q; strides of Q, K and V are positive
+ * (K and V may have a head stride of 0: one key head seen as several).
  * ------------------------------------------------------------------------------------- */
 typedef struct {
     int dtype;
@@ -359,8 +361,8 @@ typedef struct {
     deca_tokens Q, O;
     deca_cache K, V;
     const int32_t *block_table, *cu_q, *kv_lens;
-    void *workspace;     /* deca_paged_attn_workspace_bytes, 256-byte aligned; contents need no preparation.
-                            Calls that overlap in time need one each */
+    void *workspace;     /* deca_paged_attn_workspace_bytes (0: may be null), 256-byte aligned; contents need no
+                            preparation.  Calls that overlap in time need one each */
     size_t workspace_bytes;
 } deca_paged_attn_args;
 

@@ -231,6 +231,14 @@ def test_strides_and_untouched_rows(max_q):
     assert (out[45:] == 7).all() and (out[:, 0] == 7).all() and (out[:, 7] == 7).all()
 
 
+@pytest.mark.parametrize("max_q,max_kv", [(1, 100), (1, 20000), (1000, 100)])
+def test_out_may_be_q(max_q, max_kv):
+    data = make_paged([3000, 70], [40, 1], 8, 2, 64, 32, torch.bfloat16, fill=0.0)
+    want = run(*data, 32, max_q=max_q, max_kv=max_kv)
+    q = data[0].clone()
+    assert torch.equal(run(q, *data[1:], 32, max_q=max_q, max_kv=max_kv, out=q), want)
+
+
 @pytest.mark.parametrize("max_q", [1, 1000])
 def test_one_key_head_expanded(max_q):
     """A cache of one key head seen as four (a head stride of zero) is that head four times; query rows that do not

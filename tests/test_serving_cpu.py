@@ -94,15 +94,18 @@ def test_rotary_entries_refuse(native):
 
 def test_step_entry_refuses(native):
     L, p = native.lib(), 4096
-    good = dict(ctx=p, new=p, B=2, table=p, stride=4, W=4, free=p, cap=3, n_free=p, page=16, T=8, cu=p + 64, kv=p + 128, pos=p, slots=p,
-                left=p + 192, short=p)
+    k = 1024
+    good = dict(ctx=p, new=p + k, B=2, table=p + 2 * k, stride=4, W=4, free=p + 3 * k, cap=3, n_free=p + 4 * k, page=16, T=8, cu=p + 5 * k,
+                kv=p + 6 * k, pos=p + 7 * k, slots=p + 8 * k, left=p + 9 * k, short=p + 10 * k)
 
     def call(**kw):
         return L.deca_paged_step(*{**good, **kw}.values(), None)
 
     for kw, code in (({"B": 0}, -2), ({"B": 8193}, -2), ({"W": 0}, -2), ({"T": -1}, -2), ({"cap": -1}, -2), ({"page": 24}, -2),
                      ({"stride": 3}, -2), ({"W": 2**27, "stride": 2**27}, -2), ({"ctx": None}, -1), ({"free": None}, -1), ({"slots": None}, -1),
-                     ({"kv": p}, -5), ({"left": p}, -5)):
+                     ({"kv": p}, -5), ({"kv": p + 4}, -5), ({"left": p + 4 * k}, -5), ({"cu": p + k - 4}, -5), ({"pos": p + 2 * k + 16}, -5),
+                     ({"slots": p + 7 * k + 28}, -5), ({"free": p + 2 * k + 28}, -5), ({"short": p + 9 * k}, -5), ({"slots": p + 8 * k + 4}, -3), ({"ctx": p + 2}, -3),
+                     ({"pos": p + 7 * k + 1}, -3)):
         assert call(**kw) == code, kw
 
 
