@@ -11,6 +11,7 @@
 // in one warp's span and its maximum takes shuffles alone.
 // Rows beyond the registers of a CTA are streamed twice (three times for one scale a row).
 #include "common.cuh"
+#include "ptx.cuh"
 
 namespace deca {
 namespace {
@@ -35,6 +36,37 @@ struct AddNormArgs {
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Two fp32 operations in one instruction (the 8-bit forms issue in 78 % of the cycles without them).
+__device__ __forceinline__ void add_pairs(float (&a)[8], const float (&b)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) f32x2_unpack(f32x2_add(f32x2_pack(a[i], a[i + 1]), f32x2_pack(b[i], b[i + 1])), a[i], a[i + 1]);
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// y = h * rs * w
+__device__ __forceinline__ void scale_pairs(float (&h)[8], float rs, const float (&w)[8]) {
+    const uint64_t r2 = f32x2_pack(rs, rs);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2)
+        f32x2_unpack(mul_pair(mul_pair(f32x2_pack(h[i], h[i + 1]), r2), f32x2_pack(w[i], w[i + 1])), h[i], h[i + 1]);
+}
+__device__ __forceinline__ uint64_t square_pairs(const float (&h)[8], uint64_t sum) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const uint64_t p = f32x2_pack(h[i], h[i + 1]);
+        sum = f32x2_fma(p, p, sum);
+    }
+    return sum;
+}
+__device__ __forceinline__ float max3_nan_abs(float m, float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
     return r;
 }
 
@@ -144,7 +176,7 @@ __device__ __forceinline__ void store_e4m3(char *row, int span, int lane, int N,
 __device__ __forceinline__ float abs_max8(const float (&y)[8]) {
     float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(y[i]));
+    for (int i = 0; i < 8; i += 2) m = max3_nan_abs(m, y[i], y[i + 1]);
     return m;
 }
 
@@ -224,6 +256,9 @@ __global__ void __launch_bounds__(kMaxRegThreads) add_rmsnorm_reg_kernel(const A
     const char *xrow = a.x + row * a.sx * 2, *rrow = a.r + row * a.sr * 2;
     char *hrow = a.h + row * a.sh * 2, *yrow = a.y + row * a.sy * (OUT == DECA_OUT_SAME ? 2 : 1);
 
+    // fp32 pairs pay with one scale a row (16384 x 8192: 161 -> 156 us); with grouped scales they cost (165 -> 194), and
+    // the 16-bit output is at the memory's rate either way
+    constexpr bool kPairs = OUT == DECA_OUT_E4M3;
     float h[C][8];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -231,14 +266,27 @@ __global__ void __launch_bounds__(kMaxRegThreads) add_rmsnorm_reg_kernel(const A
         float r[8];
         load8<DT, V, true>(h[c], xrow, span, lane, N);
         load8<DT, V, true>(r, rrow, span, lane, N);
+        if constexpr (kPairs) {
+            add_pairs(h[c], r);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[c][i] += r[i];
+            for (int i = 0; i < 8; ++i) h[c][i] += r[i];
+        }
     }
     float ss = 0.f;
+    if constexpr (kPairs) {
+        uint64_t squares = 0ull;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c) squares = square_pairs(h[c], squares);
+        float odd;
+        f32x2_unpack(squares, ss, odd);
+        ss += odd;
+    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(h[c][i], h[c][i], ss);
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = fmaf(h[c][i], h[c][i], ss);
+    }
     ss = row_reduce<false>(ss, red[0], nw, rb * nw, wr, lane);
     const float rs = rsqrtf(fmaf(ss, a.inv_n, a.eps));
 
@@ -249,8 +297,12 @@ __global__ void __launch_bounds__(kMaxRegThreads) add_rmsnorm_reg_kernel(const A
         store8<DT, V>(hrow, span, lane, N, h[c]);
         float w[8];
         load8<DT, V, false>(w, a.w, span, lane, N);
+        if constexpr (kPairs) {
+            scale_pairs(h[c], rs, w);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[c][i] = h[c][i] * rs * w[i];
+            for (int i = 0; i < 8; ++i) h[c][i] = h[c][i] * rs * w[i];
+        }
         if constexpr (OUT == DECA_OUT_SAME)
             store8<DT, V>(yrow, span, lane, N, h[c]);
         else if constexpr (OUT == DECA_OUT_E4M3)

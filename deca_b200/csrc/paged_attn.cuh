@@ -362,7 +362,46 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
     const int lane = threadIdx.x & 31, c0 = (int)blockIdx.x;
     // part i: the CTA that starts the item keeps it in its second slot, the following ones in their first
     auto part = [&](int i) { return g.part + ((size_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats<TL::ROWS, D>; };
-    for (int row = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); row < TL::ROWS; row += gridDim.y * (kJoinThreads / 32)) {
+    const int warp = threadIdx.x >> 5, warps = kJoinThreads / 32;
+    if (it.last == c0 + 1) {
+        // two parts, the usual case: four rows of a warp with all their loads in flight
+        constexpr int R = 4, PER = D / 32;
+        const float *p0 = part(0), *p1 = part(1);
+        for (int row0 = (blockIdx.y * warps + warp) * R; row0 < TL::ROWS; row0 += gridDim.y * warps * R) {
+            float m0[R], m1[R], l0[R], l1[R], x0[R][PER], x1[R][PER];
+            auto numerators = [&](const float *p, int row, float (&x)[PER]) {
+                if constexpr (PER == 4) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + (size_t)row * D) + lane);
+                    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+                } else {
+                    const float2 v = __ldcg(reinterpret_cast<const float2 *>(p + (size_t)row * D) + lane);
+                    x[0] = v.x, x[1] = v.y;
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const size_t at = (size_t)TL::ROWS * D + row0 + i;
+                m0[i] = __ldcg(p0 + at), l0[i] = __ldcg(p0 + at + TL::ROWS);
+                m1[i] = __ldcg(p1 + at), l1[i] = __ldcg(p1 + at + TL::ROWS);
+                numerators(p0, row0 + i, x0[i]);
+                numerators(p1, row0 + i, x1[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                int tok, j;
+                if (!TL::place(g, it.n, it.tile, row0 + i, tok, j)) continue;
+                const float top = fmaxf(m0[i], m1[i]), base = top == -INFINITY ? 0.f : top;
+                const float w0 = exp2f(m0[i] - base), w1 = exp2f(m1[i] - base);
+                float acc[PER];
+#pragma unroll
+                for (int k = 0; k < PER; ++k) acc[k] = fmaf(w0, x0[i][k], w1 * x1[i][k]);
+                store_joined<DT, D>(g.o + 2 * (((long long)it.q0 + tok) * g.o_st + (long long)(it.head * g.group + j) * g.o_sh), lane, acc,
+                                    fmaf(w0, l0[i], w1 * l1[i]));
+            }
+        }
+        return;
+    }
+    for (int row = blockIdx.y * warps + warp; row < TL::ROWS; row += gridDim.y * warps) {
         int tok, j;
         if (!TL::place(g, it.n, it.tile, row, tok, j)) continue;
         float acc[D / 32], sum;

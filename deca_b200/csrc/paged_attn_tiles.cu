@@ -699,7 +699,7 @@ int launch_tiles(const PagedArgs &g, const deca_paged_attn_args &a, int sms, cud
     if (int rc = ensure_dynamic_smem(paged_tiles_kernel<DT, D>, Layout<D>::smem, configured)) return rc;
     paged_tiles_kernel<DT, D><<<(unsigned)sms, kThreads, Layout<D>::smem, st>>>(tmQ, tmK, tmV, g);
     if (cudaError_t e = cudaGetLastError()) return (int)e;
-    return launch_join<DT, D, TL>(g, (unsigned)sms, 16, st);
+    return launch_join<DT, D, TL>(g, (unsigned)sms, 8, st);
 }
 
 }  // namespace
