@@ -7,6 +7,9 @@
 // in its own shared memory and then takes its share of the tokens and of the new pages.  A page that
 // the step hands out is computed from its rank in the free list by whoever needs it and never read back
 // from the table, so the CTAs are independent of each other.
+//
+// Bound by latency: 8 requests 3.0 - 3.3 us, 512 requests with 76 800 token rows 4.8 - 5.1 us (CTAs of 1024 threads, whose
+// warp sums one thread after the other adds up, took 7.0 and 8.7).
 #include "common.cuh"
 #include "ptx.cuh"
 
