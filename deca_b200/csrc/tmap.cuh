@@ -42,7 +42,9 @@ inline int make_tmap_16bit(CUtensorMap *out, int dtype, const void *base, int ra
         uint64_t dims[4], strides[3];
         uint32_t box[4];
         int dtype, rank, swizzle;
+        int zero;  // no padding: keys are compared byte by byte
     };
+    static_assert(sizeof(Key) == 8 + 4 * 8 + 3 * 8 + 4 * 4 + 4 * 4, "no padding");
     struct Entry {
         Key key;
         CUtensorMap map;

@@ -151,6 +151,18 @@ def test_many_requests(max_q, max_kv):
     check(run(*data, 16, max_q=max_q, max_kv=max_kv), *data)
 
 
+@pytest.mark.parametrize("max_q,max_kv", [(1, 1), (1, 1000000), (1000, 1)])
+def test_more_requests_than_shared_memory_holds(max_q, max_kv):
+    """Every request has one key: its output is that key's value, to the bit."""
+    B = 17000
+    g = torch.Generator().manual_seed(0)
+    q = torch.randn(B, 2, 64, generator=g).half().cuda()
+    kc, vc = (torch.randn(B, 16, 1, 64, generator=g).half().cuda() for _ in range(2))
+    table = torch.randperm(B, generator=g).to(torch.int32).view(B, 1).cuda()
+    got = run(q, kc, vc, table, list(range(B + 1)), [1] * B, 16, max_q=max_q, max_kv=max_kv)
+    assert torch.equal(got, vc[table[:, 0].long(), 0].expand(B, 2, 64))
+
+
 @pytest.mark.parametrize("new", [1, 3])
 def test_long_ragged_batch_is_cut_between_requests(new):
     """Long contexts on more pairs than CTAs: a CTA's steps start and end inside items."""
@@ -282,12 +294,13 @@ def test_large_scores_and_raised_maxima(max_q):
     assert ((got.double() - want).abs() <= attention_bound(want, mag, q.dtype) + 2.0**-11 * mag).all()
 
 
-def test_graphs_streams_and_two_calls_at_once():
+@pytest.mark.parametrize("new", [1, 60])
+def test_graphs_streams_and_two_calls_at_once(new):
     """Two captured graphs replayed on two streams at the same time, each with work to join."""
     from deca_b200.operators import PagedAttention
 
-    sets = [make_paged([9000, 500], [1, 1], 8, 2, 128, 64, torch.bfloat16, seed=s) for s in (1, 2)]
-    op = PagedAttention(2, 8, 2, 128, 64, 1, 9000, "bfloat16")
+    sets = [make_paged([9000, 500], [new, 1], 8, 2, 128, 64, torch.bfloat16, seed=s) for s in (1, 2)]
+    op = PagedAttention(2, 8, 2, 128, 64, new, 9000, "bfloat16")
     args = [(q, kc, vc, t, i32(cu), i32(kv)) for q, kc, vc, t, cu, kv in sets]
     want = [op(*a) for a in args]
     outs = [torch.zeros_like(w) for w in want]
