@@ -47,7 +47,7 @@ def check_e4m3(q, s, y, N, group, fp32=1e-5):
 
 
 SHAPES = [(1, 1), (1, 7), (3, 8), (2, 63), (5, 64), (1, 4096), (300, 96), (297, 513), (17, 1000), (4, 8192), (301, 5000),
-          (2, 20000), (3, 32768), (2, 32776), (1, 70001)]
+          (2, 20000), (3, 32768), (2, 32776), (1, 70001), (9, 65), (300, 66), (11, 255), (8, 249), (17, 4097), (5, 16389), (9, 40002)]
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
@@ -63,7 +63,7 @@ def test_sixteen_bits(M, N, dtype):
 
 
 @pytest.mark.parametrize("group", [0, 32, 64, 128, 256])
-@pytest.mark.parametrize("M,N", [(1, 1), (3, 100), (5, 256), (300, 513), (17, 4096), (301, 5000), (2, 33000), (2, 32769)])
+@pytest.mark.parametrize("M,N", [(1, 1), (3, 100), (5, 256), (300, 513), (17, 4096), (301, 5000), (2, 33000), (2, 32769), (13, 1003), (9, 70), (300, 129)])
 def test_eight_bits(M, N, group):
     from deca_b200.operators import AddRMSNorm
 
@@ -74,12 +74,13 @@ def test_eight_bits(M, N, group):
     check_e4m3(q, s, want_y, N, group, 7e-5 if N > 32768 else 1e-5)
 
 
-@pytest.mark.parametrize("N,offset", [(512, 0), (512, 1), (511, 0), (4096, 8)])
-def test_strides_and_alignment(N, offset):
+@pytest.mark.parametrize("extra", [40, 37])
+@pytest.mark.parametrize("N,offset", [(512, 0), (512, 1), (511, 0), (4096, 8), (1000, 4)])
+def test_strides_and_alignment(N, offset, extra):
     """Rows that are slices of wider tensors, aligned for wide accesses and not; neighbours stay."""
     from deca_b200.operators import AddRMSNorm
 
-    M, wide = 9, N + 40
+    M, wide = 9, N + extra
     g = torch.Generator().manual_seed(1)
     big = [torch.randn(M, wide, generator=g).half().cuda() for _ in range(4)]
     x, res, h, y = (b[:, offset : offset + N] for b in big)
@@ -94,7 +95,7 @@ def test_strides_and_alignment(N, offset):
     assert torch.equal(x, before[0][:, offset : offset + N]) and torch.equal(res, before[1][:, offset : offset + N])
 
 
-@pytest.mark.parametrize("N", [1000, 40000])
+@pytest.mark.parametrize("N", [1000, 1001, 40000, 40001])
 def test_in_place(N):
     """The residual updated in place and y over x give the same bits as tensors of their own."""
     from deca_b200.operators import AddRMSNorm
