@@ -14,8 +14,9 @@
 // Bound by HBM (measured copy rate 6.57 TB/s).  bf16, device time: 16384 x 4096 to 16 bits 81.0 us = 6.63 TB/s,
 // 8000 x 12000 117.8 us = 6.52; to e4m3 16384 x 8192 per row 155.5 us = 6.04 TB/s, per 128 columns 165.3 us = 5.71
 // (issue slots 78 % busy: the conversions and maxima show), 1021 x 5000 per row 9.2 us; rows of 1001 elements (2-byte
-// accesses) 3.25 TB/s.  16 x 4096: 2.3 us, launch latency; there a warp takes one span instead of two (256 x 8192
-// 3.9 us), which is what shortens the chain of loads.
+// accesses) 3.25 TB/s, 19.7 us at 8000 x 1001 (16-byte accesses shifted through shared memory: 23.2).  16 x 4096: 2.3 us,
+// launch latency; there a warp takes one span instead of two (256 x 8192 3.9 us), which is what shortens the chain of
+// loads.
 #include "common.cuh"
 #include "ptx.cuh"
 

@@ -21,7 +21,8 @@
 // heads a key head) 421 us = 1.14 PFLOPS (the dense persistent schedule: 1.09 sustained, 1.28 in isolated launches), 1 x 8192 553,
 // 4 x 4096 with 16 equal heads 341 (D = 64: 284), a ragged batch of 9 at D = 64 182.
 // Tried and slower: two warps per 32 rows (445 us on the first of these), an issuing thread per tile (567), P in
-// columns of its own at D = 64, which tensor memory has room for, so that scores run ahead (193 on the last).
+// columns of its own at D = 64, which tensor memory has room for, so that scores run ahead (193 on the last); no gain:
+// the next item's first scores issued before the last product (426 and 185).
 #include <cuda.h>
 
 #include "fa_softmax.cuh"
