@@ -27,16 +27,20 @@ bool use_tiles(const deca_paged_attn_args &a) {
     return (int64_t)a.max_q * (a.H_q / a.H_kv) > 32 && a.scale > 0.f;  // the tiles keep maxima of unscaled scores
 }
 // Whether the streaming schedule cuts items.  Whole, a (request, key head) pair is one CTA's and costs nothing but
-// its keys; cut, the CTAs share the keys evenly, which costs 10 - 15 us of partial results and joining.  Measured
-// (D = 128, 8 key heads, whole / cut): 16 x 2000 keys 28.7 / 31.5 us, 32 x 500 .. 2500 43 / 48, 256 x 100 .. 500
-// 67 / 87; but 4 x 4000 49 / 21, 1 x 8192 93 / 18, 64 x 1000 .. 8191 226 / 214.
+// its keys; cut, the CTAs share the keys evenly, which costs 3 - 10 us of partial results and joining.  Measured
+// (D = 128, 8 key heads, 16 rows, whole / cut): 16 x 2000 keys 28.3 / 31.8 us, 37 x 3000 72.9 / 75.2, 256 x 100 .. 500
+// 66.8 / 72.8; but 4 x 4000 49 / 21, 1 x 8192 93 / 18, 64 x 0 .. 3000 90.6 / 77.8, 100 x 0 .. 1500 65.1 / 62.6, 100 x
+// 1000 .. 4000 193 / 172; D = 64: 64 x 0 .. 4000 67.8 / 59.4.  More pairs than CTAs gain at any length where the last
+// round is nearly empty (150 x 0 .. 3000, 2 key heads, 71.6 / 53.2), and with small CTAs (D = 64) or 32 rows only there:
+// 100 x 0 .. 2000 (16 heads of 64) 76.8 / 85.5, 200 x 0 .. 2000 (32 rows) 225 / 294.
 bool use_cuts(const deca_paged_attn_args &a, int sms) {
     if (a.max_kv <= 768) return false;
     const double pairs = (double)a.B * a.H_kv, ctas = paged_rows_ctas(a.D, row_tiles(a), sms);
     if (8 * pairs < 3 * ctas) return true;
-    // microseconds of reading half of the longest contexts, and the share of them that the last round idles
-    const double us = pairs * a.max_kv * a.D * 2.0 / 6.5e6, rounds = std::ceil(pairs / ctas);
-    return pairs <= ctas ? us > 60 : us * (rounds * ctas / pairs - 1.0) > 15;
+    // microseconds of reading half of the longest contexts
+    const double us = pairs * a.max_kv * a.D * 2.0 / 6.5e6;
+    if (us > 36 && (pairs <= ctas || (a.D == 128 && row_tiles(a) == 1))) return true;
+    return pairs > ctas && us * (std::ceil(pairs / ctas) * ctas / pairs - 1.0) > 15;  // the last round's idle share of them
 }
 // Tensor maps want strides that advance.  A dimension of one element may have any; a head stride of zero (one key head
 // expanded to several) becomes a dimension of one element.

@@ -4,10 +4,11 @@
 // Lengths live on the device, so the division is made there.  An item is one tile of query rows of one
 // request and key head; row i of a tile packs token i / group and query head i % group of the key head, so
 // all rows of an item read the same keys.  An item costs as many steps as it has key tiles (one at least: a
-// row that sees no key is still written).  With U steps in all and G CTAs, CTA c takes the steps
-// [U c / G, U (c + 1) / G) of the concatenated items: every CTA gets the same number of key tiles, whatever
-// the lengths are.  An item that is cut leaves one partial result per CTA (fp32 numerators, maximum and
-// sum per row), and a second kernel joins them in the order of the keys, so results do not depend on timing.
+// row that sees no key is still written), and its start and end as much as a few more (kItemSteps), which come
+// first.  With U steps in all and G CTAs, CTA c takes the steps [U c / G, U (c + 1) / G) of the concatenated
+// items: every CTA gets the same share, whatever the lengths are.  An item that is cut leaves one partial result
+// per CTA (fp32 numerators, maximum and sum per row); they are joined in the order of the keys, so results do not
+// depend on timing.
 #pragma once
 
 #include "ptx.cuh"
@@ -72,6 +73,9 @@ __device__ __forceinline__ int keys_until(const ReqView &v, int last_token) {
 template <int ROWS_, int KEYS>
 struct PackedRows {
     static constexpr int ROWS = ROWS_;
+    // Device time without / with 2 / with 4 / with 6 steps for an item's start and end: 64 requests of 1000 .. 8191 keys
+    // (D = 128) 210 / 204 / 202 / 203 us, 200 of 1 .. 8000 keys 516 / 497 / 488 / 491.
+    static constexpr int kItemSteps = 4;
     // token of the request and head of the group in `row` of a tile; false: the row is not in use
     static __device__ __forceinline__ bool place(const PagedArgs &g, int n, int tile, int row, int &tok, int &j) {
         const unsigned long long packed = (unsigned long long)tile * ROWS + row;
@@ -93,8 +97,8 @@ struct PackedRows {
         return max((keys_until(v, last_token(g, v, tile)) + KEYS - 1) / KEYS, 1);
     }
     static __device__ __forceinline__ long long head_steps(const PagedArgs &g, const ReqView &v) {
-        long long s = 0;
         const int n = tiles(g, v);
+        long long s = (long long)n * kItemSteps;
         for (int t = 0; t < n; ++t) s += steps(g, v, t);
         return s;
     }
@@ -104,6 +108,10 @@ struct PackedRows {
 template <int KEYS>
 struct TokenTiles {
     static constexpr int ROWS = 256;
+    // Device time without / with 1 / 2 / 3 / 4 steps: 9 requests of 188 .. 700 tokens and up to 5000 keys (D = 64)
+    // 187 / 151 / 134 / 139 / 142 us, 20 of up to 700 tokens (D = 128) 362 / 302 / 290 / 294 / 300, one of 8192 tokens
+    // 547 / 507 / 488 / 494 / 501, 4 of 4096 with equal heads 342 / 329 / 332 / 319 / 324.
+    static constexpr int kItemSteps = 2;
     static __device__ __forceinline__ int tokens(const PagedArgs &g) { return g.tile_tokens; }  // of one of the two
     static __device__ __forceinline__ bool place(const PagedArgs &g, int n, int tile, int row, int &tok, int &j) {
         const int r = row & 127, t = r / g.group;
@@ -120,8 +128,8 @@ struct TokenTiles {
         return max((keys_until(v, last) + KEYS - 1) / KEYS, 1);
     }
     static __device__ __forceinline__ long long head_steps(const PagedArgs &g, const ReqView &v) {
-        long long s = 0;
         const int n = tiles(g, v);
+        long long s = (long long)n * kItemSteps;
         for (int t = 0; t < n; ++t) s += steps(g, v, t);
         return s;
     }
@@ -131,11 +139,11 @@ struct TokenTiles {
 struct WorkPos {
     int req, head, tile;
     int step;  // first step of the current item that is this CTA's
-    int left;  // steps this CTA still has to take
+    int left;  // steps this CTA still has to take, starts of later items included
 };
 // The CTA's range in the list; kept in shared memory, read where an item is cut.
 struct WorkShare {
-    long long begin, end, total;  // its first step, one past its last; steps in all
+    long long end, total;  // one past its last step; steps in all
     int ctas;              // CTAs that share the work
     WorkPos first;
     long long warp_sum[32];
@@ -184,12 +192,13 @@ __device__ __forceinline__ bool find_work(const PagedArgs &g, WorkPos &out, Work
             const int head = (int)((u0 - at) / per_head);
             at += per_head * head;
             int tile = 0;
-            for (int s; u0 >= at + (s = TL::steps(g, v, tile)); ++tile) at += s;
+            for (int s; u0 >= at + (s = TL::kItemSteps + TL::steps(g, v, tile)); ++tile) at += s;
             const unsigned long long u1 = total * (c + 1) / ctas;
-            share->first.req = r, share->first.head = head, share->first.tile = tile;
-            share->first.step = (int)(u0 - at);
-            share->first.left = (int)min(u1 - u0, 2147483647ull);
-            share->begin = (long long)u0;
+            at += TL::kItemSteps;
+            const unsigned long long from = max(u0, at);  // of a range that begins in an item's start the item is whole
+            share->first.req = from < u1 ? r : -1, share->first.head = head, share->first.tile = tile;
+            share->first.step = (int)(from - at);
+            share->first.left = (int)min(u1 - from, 2147483647ull);
             share->end = (long long)u1;
             share->total = (long long)total;
             share->ctas = (int)ctas;
@@ -256,9 +265,11 @@ __device__ __forceinline__ int find_part(const PagedArgs &g, WorkPos &w, ReqView
     return 1;
 }
 
-// Moves on to the next item of the list; false behind the last one.
+// Moves on to the next item of the list; false where the CTA's range ends before its first step.
 template <typename TL>
 __device__ __forceinline__ bool next_item(const PagedArgs &g, WorkPos &w, ReqView &v) {
+    w.left -= TL::kItemSteps;
+    if (w.left <= 0) return false;
     w.step = 0;
     if (++w.tile < TL::tiles(g, v)) return true;
     w.tile = 0;

@@ -9,11 +9,11 @@
 // rows would be idle in 7 of 8 lanes, and the tensor work is a tenth of the memory time either way:
 // bytes of K and V bound this kernel.
 //
-// Measured (bf16, D = 128, 32 query and 8 key heads, pages of 16, device time): 64 requests of 1000 .. 8191 keys 215 us =
-// 6.03 TB/s (92 % of the measured copy rate; 19 % of the tensor pipe), 16 x 2000 28.7 us, 32 x 500 .. 2500 42.6,
+// Measured (bf16, D = 128, 32 query and 8 key heads, pages of 16, device time): 64 requests of 1000 .. 8191 keys 205 us =
+// 6.32 TB/s (96 % of the measured copy rate; 20 % of the tensor pipe), 100 x 1000 .. 4000 171, 16 x 2000 28.4 us, 32 x 500 .. 2500 42.6,
 // 256 x 100 .. 500 67 (4.6 TB/s: the start and end of an item, 5 us, show), 1 x 8192 16.9, 1 x 333 (D = 64, 16 equal
-// heads) 6.2.  A TMA producer warp ahead of four consumers measured 205 and 61.5 us on the first and fourth of these
-// but 38 and 48 on the second and third (the warps meet twice a step), and with independent consumers it was
+// heads) 6.2.  A TMA producer warp ahead of four consumers gained 5 and 8 % on the first case and on the 256 requests
+// but took 38 and 48 us on 16 x 2000 and 32 x 500 .. 2500 (the warps meet twice a step), and with independent consumers it was
 // slower everywhere (two barrier waits a step instead of one own copy group).
 //
 // The running maximum moves only when a score exceeds it by 2^8 (it then rescales the numerators);

@@ -151,6 +151,20 @@ def test_many_requests(max_q, max_kv):
     check(run(*data, 16, max_q=max_q, max_kv=max_kv), *data)
 
 
+@pytest.mark.parametrize("max_q,max_kv", [(1, 1000000), (1000, 1)])
+@pytest.mark.parametrize("B", [19, 37, 75, 110, 149, 200, 301, 600])
+@pytest.mark.parametrize("longest", [1, 70, 3000])
+def test_ranges_shorter_than_an_item_and_its_start(longest, B, max_q, max_kv):
+    """A CTA's range may begin or end in what an item's start costs, or hold no key tile at all."""
+    g = torch.Generator().manual_seed(B + longest)
+    kv = torch.randint(0, 3, (B,), generator=g).tolist()
+    kv[0], kv[B // 2], kv[-1] = longest, longest // 2 + 1, longest
+    data = make_paged(kv, [min(k, 1) for k in kv], 4, 4, 64, 16, torch.float16)
+    got = run(*data, 16, max_q=max_q, max_kv=max_kv)
+    check(got, *data)
+    assert torch.equal(got, run(*data, 16, max_q=max_q, max_kv=max_kv))
+
+
 @pytest.mark.parametrize("max_q,max_kv", [(1, 1), (1, 1000000), (1000, 1)])
 def test_more_requests_than_shared_memory_holds(max_q, max_kv):
     """Every request has one key: its output is that key's value, to the bit."""
