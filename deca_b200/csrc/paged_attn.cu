@@ -22,9 +22,15 @@ bool cache_ok(const deca_cache &c) {
 // 16 rows each of the streaming schedule
 int row_tiles(const deca_paged_attn_args &a) { return (int64_t)a.max_q * (a.H_q / a.H_kv) <= 16 ? 1 : 2; }
 
-// The tensor-core tiles take what has more than 32 query rows per request and key head.
-bool use_tiles(const deca_paged_attn_args &a) {
-    return (int64_t)a.max_q * (a.H_q / a.H_kv) > 32 && a.scale > 0.f;  // the tiles keep maxima of unscaled scores
+// The tensor-core tiles take what has more than 32 query rows per request and key head, and from 17 rows on what the
+// streaming schedule divides badly.  Measured with 17 .. 32 rows (D = 128, 8 key heads, streamed / tiles): few pairs of
+// long contexts, 8 x 4000 keys 68 / 49 us, 1 x 8192 53 / 23, 9 x 1500 46 / 36 (D = 64: 1 x 8192 34 / 19, 4 x 4000 25 /
+// 26), but 2 x 500 15.8 / 16.0; more pairs than CTAs, 64 x 2000 .. 8000 397 / 354, 100 x 0 .. 3000 202 / 170, but
+// 200 x 0 .. 2000 225 / 242 and D = 64 64 x 2000 .. 8000 191 / 265.  Between them, 32 x 3000 87 / 119.
+bool use_tiles(const deca_paged_attn_args &a, int sms) {
+    const int64_t rows = (int64_t)a.max_q * (a.H_q / a.H_kv), pairs = (int64_t)a.B * a.H_kv;
+    if (rows <= 16 || !(a.scale > 0.f)) return false;  // the tiles keep maxima of unscaled scores
+    return rows > 32 || (2 * pairs <= sms && a.max_kv > 768) || (a.D == 128 && pairs > 2 * (int64_t)sms && a.max_kv > 2048);
 }
 // Whether the streaming schedule cuts items.  Whole, a (request, key head) pair is one CTA's and costs nothing but
 // its keys; cut, the CTAs share the keys evenly, which costs 3 - 10 us of partial results and joining.  Measured
@@ -94,7 +100,7 @@ extern "C" int deca_paged_attn_workspace_bytes(const deca_paged_attn_args *a, si
     DeviceInfo di;
     if (int rc = current_device_info(&di)) return rc;
     *bytes = use_cuts(*a, di.sms) ? paged_rows_workspace(a->D, row_tiles(*a), di.sms) : 0;
-    if (use_tiles(*a) && paged_tiles_workspace(a->D, di.sms) > *bytes) *bytes = paged_tiles_workspace(a->D, di.sms);
+    if (use_tiles(*a, di.sms) && paged_tiles_workspace(a->D, di.sms) > *bytes) *bytes = paged_tiles_workspace(a->D, di.sms);
     return DECA_OK;
 }
 
@@ -122,7 +128,7 @@ extern "C" int deca_paged_attn(const deca_paged_attn_args *a, void *stream) {
     g.sl2 = a->scale * kLog2e;
     g.status = device_status_ptr();
     if (!g.status) return (int)cudaErrorUnknown;
-    if (use_tiles(*a) && query_strides(*a, g.q_st, g.q_sh)) {
+    if (use_tiles(*a, di.sms) && query_strides(*a, g.q_st, g.q_sh)) {
         g.min_steps = 2;
         g.max_parts = 1 << 20;
         return paged_tiles_launch(*a, g, di.sms, static_cast<cudaStream_t>(stream));

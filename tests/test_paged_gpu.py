@@ -188,6 +188,19 @@ def test_long_ragged_batch_is_cut_between_requests(new):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("B,H_kv,D,max_kv", [(3, 2, 128, 1500), (3, 2, 64, 1500), (3, 2, 128, 700), (160, 2, 128, 3000), (160, 2, 64, 3000), (160, 2, 128, 900)])
+def test_short_guesses(B, H_kv, D, max_kv):
+    """17 to 32 rows a key head: few long contexts, many, and shorter ones."""
+    g = torch.Generator().manual_seed(B + D)
+    new = torch.randint(1, 8, (B,), generator=g).tolist()
+    new[0] = 7
+    kv = [n + k for n, k in zip(new, torch.randint(0, min(max_kv, 1200) - 8, (B,), generator=g).tolist())]
+    data = make_paged(kv, new, 4 * H_kv, H_kv, D, 16, torch.bfloat16)
+    got = run(*data, 16, max_kv=max_kv)
+    check(got, *data)
+    assert torch.equal(got, run(*data, 16, max_kv=max_kv))
+
+
 @pytest.mark.parametrize("H_q,H_kv,new", [(128, 1, 2), (200, 2, 3), (24, 1, 1), (40, 2, 70), (31, 1, 33)])
 def test_wide_and_odd_groups(H_q, H_kv, new):
     data = make_paged([1500, 77], [new, 1], H_q, H_kv, 64, 64, torch.float16)
