@@ -10,7 +10,7 @@
 // bytes of K and V bound this kernel.
 //
 // Measured (bf16, D = 128, 32 query and 8 key heads, pages of 16, device time): 64 requests of 1000 .. 8191 keys 205 us =
-// 6.32 TB/s (96 % of the measured copy rate; 20 % of the tensor pipe), 100 x 1000 .. 4000 171, 16 x 2000 28.4 us, 32 x 500 .. 2500 42.6,
+// 6.32 TB/s (96 % of the measured copy rate; 19 % of the tensor pipe), 100 x 1000 .. 4000 171, 16 x 2000 28.4 us, 32 x 500 .. 2500 42.6,
 // 256 x 100 .. 500 67 (4.6 TB/s: the start and end of an item, 5 us, show), 1 x 8192 16.9, 1 x 333 (D = 64, 16 equal
 // heads) 6.2.  A TMA producer warp ahead of four consumers gained 5 and 8 % on the first case and on the 256 requests
 // but took 38 and 48 us on 16 x 2000 and 32 x 500 .. 2500 (the warps meet twice a step), and with independent consumers it was
