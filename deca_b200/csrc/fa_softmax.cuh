@@ -83,21 +83,30 @@ __device__ __forceinline__ float fa_exp_tile(uint32_t tS, uint32_t p_base, int r
 }
 
 // 2^x for two scores on the FMA pipe instead of the exp2 unit (x = s * sl2 - ms):
-//   t = sat(x / 256 + 126 / 256) clamps to x' = 256 t - 126 in [-126, 130) (one saturating fma per
-//   score: what lies below 2^-126 counts as 2^-126), r = x' + 1.5 * 2^23 rounds x' to the nearest
-//   integer j in r's low mantissa bits, a degree-3 polynomial (relative error 7.6e-5, a sixth of
-//   an fp16 ulp) gives 2^(x' - j) on [-0.5, 0.5], and one integer multiply-add puts j into the
-//   exponent (r's bits times 2^23 is j * 2^23 modulo 2^32).  The additions and the polynomial
-//   run as packed pairs.
+//   t = sat(x / 128 + 112 / 128) clamps to x' = 128 t - 112 in [-112, 16] (one saturating fma per
+//   score), r = x' + 1.5 * 2^23 rounds x' to the nearest integer j in r's low mantissa bits, a
+//   degree-3 polynomial (relative error 7.6e-5, a sixth of an fp16 ulp) gives 2^(x' - j) on
+//   [-0.5, 0.5], and one integer multiply-add puts j into the exponent (r's bits times 2^23 is
+//   j * 2^23 modulo 2^32).  The additions and the polynomial run as packed pairs.
+// The ends of the window: what lies below 2^-112 counts as 2^-112 (kFaPolyLeast), and what lies above 2^16 as 2^16,
+// far over the sum limit, so that the vote sends the warp to the exact pass.  A window that ends above
+// 2^128 would let j run over the exponent's eight bits, and a score 89 above the maximum (129 / log2 e) would come out as
+// a negative number with the sum none the wiser.  A width of a power of two makes sl2 / 128 exact.
+constexpr float kFaPolyWidth = 128.0f, kFaPolyBottom = 112.0f;
+// The polynomial's constant term (0x3F7FFB43) times 2^-112, bit for bit what the window's lower end comes out as.
+constexpr float kFaPolyLeast = 0x1.fff686p-113f;
 struct FaPolyConst {
-    float sl2_256, off;  // sl2 / 256, 126 / 256 - ms / 256
+    float scale, off;  // sl2 / 128, 112 / 128 - ms / 128
 };
+__device__ __forceinline__ FaPolyConst fa_poly_const(float sl2, float ms) {
+    return {sl2 * (1.0f / kFaPolyWidth), kFaPolyBottom / kFaPolyWidth - ms * (1.0f / kFaPolyWidth)};
+}
 __device__ __forceinline__ void fa_exp2_poly_pair(float s0, float s1, const FaPolyConst &k, float &p0, float &p1) {
     float t0, t1;
-    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(t0) : "f"(s0), "f"(k.sl2_256), "f"(k.off));
-    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(t1) : "f"(s1), "f"(k.sl2_256), "f"(k.off));
+    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(t0) : "f"(s0), "f"(k.scale), "f"(k.off));
+    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(t1) : "f"(s1), "f"(k.scale), "f"(k.off));
     constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
-    const uint64_t x = f32x2_fma(f32x2_pack(t0, t1), f32x2_pack(256.0f, 256.0f), f32x2_pack(-126.0f, -126.0f));
+    const uint64_t x = f32x2_fma(f32x2_pack(t0, t1), f32x2_pack(kFaPolyWidth, kFaPolyWidth), f32x2_pack(-kFaPolyBottom, -kFaPolyBottom));
     const uint64_t r = f32x2_add(x, f32x2_pack(kMagic, kMagic));
     const uint64_t j = f32x2_add(r, f32x2_pack(-kMagic, -kMagic));
     const uint64_t f = f32x2_fma(j, f32x2_pack(-1.0f, -1.0f), x);
@@ -158,7 +167,7 @@ __device__ __forceinline__ float fa_exp_tile_hold(uint32_t tS, int col0, int row
                                                   uint32_t (&pk)[BC / 2]) {
     constexpr int kChunks = BC / 32;
     const uint64_t sl2x2 = f32x2_pack(sl2, sl2), nmsx2 = f32x2_pack(-ms, -ms);
-    const FaPolyConst pc = {sl2 * (1.0f / 256.0f), 126.0f / 256.0f - ms * (1.0f / 256.0f)};
+    const FaPolyConst pc = fa_poly_const(sl2, ms);
     uint64_t sum2[2] = {0ull, 0ull};
     uint32_t v[2][32];
     tmem_ld_32x32b_x32(tS, v[0]);

@@ -60,11 +60,8 @@ struct RingPos {
     uint32_t par;
 };
 
-// What the polynomial share makes of -inf: its constant term with 2^-126 put into the exponent (0x3F7FFB43 less
-// 126 << 23).  Taken off every polynomial value, it leaves a masked score exactly zero.
-constexpr float kPolyLeast = 0x1.ffed0cp-127f;
-
-// Exponentials of 32 scores against the maximum's term: packed to 16 bits, summed in fp32.  A masked score is -inf.
+// Exponentials of 32 scores against the maximum's term: packed to 16 bits, summed in fp32.  A masked score is -inf;
+// kFaPolyLeast, what the polynomial share makes of it, is taken off every value of that share, which leaves it exactly zero.
 template <int DT, int EVERY>
 __device__ __forceinline__ void exp_chunk32(const uint32_t (&v)[32], uint64_t sl2x2, uint64_t nmsx2, const FaPolyConst &pc,
                                             uint64_t (&sum2)[2], uint32_t *pk) {
@@ -74,7 +71,7 @@ __device__ __forceinline__ void exp_chunk32(const uint32_t (&v)[32], uint64_t sl
         float p0, p1;
         if (EVERY > 0 && i % (EVERY > 0 ? EVERY : 1) == (EVERY > 0 ? EVERY : 1) - 1) {
             fa_exp2_poly_pair(s0, s1, pc, p0, p1);
-            f32x2_unpack(f32x2_add(f32x2_pack(p0, p1), f32x2_pack(-kPolyLeast, -kPolyLeast)), p0, p1);
+            f32x2_unpack(f32x2_add(f32x2_pack(p0, p1), f32x2_pack(-kFaPolyLeast, -kFaPolyLeast)), p0, p1);
         } else {
             float x0, x1;
             f32x2_unpack(f32x2_fma(f32x2_pack(s0, s1), sl2x2, nmsx2), x0, x1);
@@ -97,7 +94,7 @@ __device__ __forceinline__ float max32(const uint32_t (&v)[32]) {
 template <int DT, int EVERY>
 __device__ __forceinline__ float exp_row(uint32_t tS, float sl2, float ms, uint32_t (&pk)[kBc / 2]) {
     const uint64_t sl2x2 = f32x2_pack(sl2, sl2), nmsx2 = f32x2_pack(-ms, -ms);
-    const FaPolyConst pc = {sl2 * (1.0f / 256.0f), 126.0f / 256.0f - ms * (1.0f / 256.0f)};
+    const FaPolyConst pc = fa_poly_const(sl2, ms);
     uint64_t sum2[2] = {0ull, 0ull};
     uint32_t v[2][32];
     tmem_ld_32x32b_x32(tS, v[0]);
