@@ -88,13 +88,11 @@ __device__ __forceinline__ float fa_exp_tile(uint32_t tS, uint32_t p_base, int r
 //   degree-3 polynomial (relative error 7.6e-5, a sixth of an fp16 ulp) gives 2^(x' - j) on
 //   [-0.5, 0.5], and one integer multiply-add puts j into the exponent (r's bits times 2^23 is
 //   j * 2^23 modulo 2^32).  The additions and the polynomial run as packed pairs.
-// The ends of the window: what lies below 2^-112 counts as 2^-112 (kFaPolyLeast), and what lies above 2^16 as 2^16,
+// The ends of the window: what lies below 2^-112 counts as 2^-112, and what lies above 2^16 as 2^16,
 // far over the sum limit, so that the vote sends the warp to the exact pass.  A window that ends above
 // 2^128 would let j run over the exponent's eight bits, and a score 89 above the maximum (129 / log2 e) would come out as
 // a negative number with the sum none the wiser.  A width of a power of two makes sl2 / 128 exact.
 constexpr float kFaPolyWidth = 128.0f, kFaPolyBottom = 112.0f;
-// The polynomial's constant term (0x3F7FFB43) times 2^-112, bit for bit what the window's lower end comes out as.
-constexpr float kFaPolyLeast = 0x1.fff686p-113f;
 struct FaPolyConst {
     float scale, off;  // sl2 / 128, 112 / 128 - ms / 128
 };

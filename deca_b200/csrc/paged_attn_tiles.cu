@@ -60,23 +60,18 @@ struct RingPos {
     uint32_t par;
 };
 
-// Exponentials of 32 scores against the maximum's term: packed to 16 bits, summed in fp32.  A masked score is -inf;
-// kFaPolyLeast, what the polynomial share makes of it, is taken off every value of that share, which leaves it exactly zero.
-template <int DT, int EVERY>
-__device__ __forceinline__ void exp_chunk32(const uint32_t (&v)[32], uint64_t sl2x2, uint64_t nmsx2, const FaPolyConst &pc,
-                                            uint64_t (&sum2)[2], uint32_t *pk) {
+// Exponentials of 32 scores against the maximum's term: packed to 16 bits, summed in fp32.  A masked score is -inf,
+// its exponential exactly zero; a NaN reaches the sum.  All of them on the exp2 unit, at D = 64 too: with every fourth
+// pair as a polynomial on the FMA pipe (which pays in the dense kernel) 9 ragged requests took 134 us instead of 128, 4 x 512
+// tokens behind 8192 129 instead of 123, 4 x 4096 265 instead of 258.
+template <int DT>
+__device__ __forceinline__ void exp_chunk32(const uint32_t (&v)[32], uint64_t sl2x2, uint64_t nmsx2, uint64_t (&sum2)[2],
+                                            uint32_t *pk) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const float s0 = __uint_as_float(v[2 * i]), s1 = __uint_as_float(v[2 * i + 1]);
-        float p0, p1;
-        if (EVERY > 0 && i % (EVERY > 0 ? EVERY : 1) == (EVERY > 0 ? EVERY : 1) - 1) {
-            fa_exp2_poly_pair(s0, s1, pc, p0, p1);
-            f32x2_unpack(f32x2_add(f32x2_pack(p0, p1), f32x2_pack(-kFaPolyLeast, -kFaPolyLeast)), p0, p1);
-        } else {
-            float x0, x1;
-            f32x2_unpack(f32x2_fma(f32x2_pack(s0, s1), sl2x2, nmsx2), x0, x1);
-            p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-        }
+        float x0, x1;
+        f32x2_unpack(f32x2_fma(f32x2_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), sl2x2, nmsx2), x0, x1);
+        const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
         sum2[i & 1] = f32x2_add(sum2[i & 1], f32x2_pack(p0, p1));
         pk[i] = Pack16<DT>::pack(p0, p1);
     }
@@ -91,10 +86,9 @@ __device__ __forceinline__ float max32(const uint32_t (&v)[32]) {
 
 // Exponentials of the whole row into registers; returns their sum.  The next 32 columns are on their way from
 // tensor memory while the current ones are processed.
-template <int DT, int EVERY>
+template <int DT>
 __device__ __forceinline__ float exp_row(uint32_t tS, float sl2, float ms, uint32_t (&pk)[kBc / 2]) {
     const uint64_t sl2x2 = f32x2_pack(sl2, sl2), nmsx2 = f32x2_pack(-ms, -ms);
-    const FaPolyConst pc = fa_poly_const(sl2, ms);
     uint64_t sum2[2] = {0ull, 0ull};
     uint32_t v[2][32];
     tmem_ld_32x32b_x32(tS, v[0]);
@@ -102,7 +96,7 @@ __device__ __forceinline__ float exp_row(uint32_t tS, float sl2, float ms, uint3
 #pragma unroll
     for (int c = 0; c < kBc / 32; ++c) {
         if (c + 1 < kBc / 32) tmem_ld_32x32b_x32(tS + (c + 1) * 32, v[(c + 1) & 1]);
-        exp_chunk32<DT, EVERY>(v[c & 1], sl2x2, nmsx2, pc, sum2, &pk[c * 16]);
+        exp_chunk32<DT>(v[c & 1], sl2x2, nmsx2, sum2, &pk[c * 16]);
         if (c + 1 < kBc / 32) tmem_ld_wait_regs(v[(c + 1) & 1]);
     }
     float a0, a1, b0, b1;
@@ -143,7 +137,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, float sl2
     {
         // held in registers until the vote: storing P overwrites the scores that a second pass would need
         uint32_t pk[kBc / 2];
-        const float sum = exp_row<DT, kFaPolyEveryFor<D>>(tS, sl2, m == -INFINITY ? 0.f : m * sl2, pk);
+        const float sum = exp_row<DT>(tS, sl2, m == -INFINITY ? 0.f : m * sl2, pk);
         if (!__any_sync(0xFFFFFFFFu, !(sum <= kFaSumLimit))) {
 #pragma unroll
             for (int h = 0; h < kBc / 64; ++h) {

@@ -102,3 +102,26 @@ def test_dense_one_key_far_above(delta, D, S, persistent, causal):
             want, mag = formula(q[0, h], k[0, h], v[0, h], 8.0 / D, 0 if causal else None)
             bad = ~((got[0, h].double() - want).abs() <= attention_bound(want, mag, q.dtype))
             assert not bad.any(), f"key {base + h}: rows {bad.any(-1).nonzero().flatten().tolist()[:9]}"
+
+
+# ---------------------------------------------------------------------------- keys that are not finite
+def special_keys(kv, new, base, value, D, dtype):
+    """Requests of ordinary data; in request r one element of key base + r is `value`, where q is 1."""
+    data = make_paged([kv] * 8, [new] * 8, 2, 1, D, 64, dtype, seed=base + 1)
+    q, kc, vc, table, _, _ = data
+    q[..., 5] = 1.0
+    for r in range(8):
+        set_key(kc, table, r, base + r, value, 64, 5)
+    return data
+
+
+@pytest.mark.parametrize("max_q,max_kv", SCHEDULES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_paged_key_that_is_not_finite(value, D, dtype, max_q, max_kv):
+    """A visible key with a NaN or a score of +inf makes its rows NaN, as the formula does; a score of -inf has no
+    weight; rows that do not see the key do not notice."""
+    for kv, new, base in PLACES:
+        data = special_keys(kv, new, base, value, D, dtype)
+        compare(run_paged(data, 64, max_q, max_kv, D**-0.5), data, D**-0.5)
