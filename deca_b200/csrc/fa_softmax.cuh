@@ -123,18 +123,30 @@ __device__ __forceinline__ void fa_exp2_poly_pair(float s0, float s1, const FaPo
 // Share of the exponentials of an unmasked tile that is taken on the FMA pipe: every EVERY-th pair
 // of scores (0: none).  At D = 64 the exp2 unit alone bounds the kernel (half the tensor work per
 // exponential) and a share on the FMA pipe pays: 682 -> 728 ... 747 TFLOPS back to back and 700 -> 798
-// in isolated launches with every fourth pair (every fifth or eighth measure the same, every third
-// 708, every second 684).  At D = 128, where the step is a dependency chain and the pass only a part
-// of it, the longer instruction stream costs what the unit gains (1 147 -> 1 143, 1 282 -> 1 258).
+// in isolated launches with every fourth pair (every third 708, every second 684).  With the test for NaN every
+// fifth is the best: 1 x 16 x 4096 x 64 takes 104.8 us (causal 56.6) against 106.2 (56.9) with every fourth, 106.9 with every
+// sixth, 106.3 with every eighth and 116.5 (61.9) with none; every fourth without the test took 102.4 (55.7).  At D = 128,
+// where the step is a dependency chain and the pass only a part of it, the longer instruction stream costs
+// what the unit gains (1 147 -> 1 143, 1 282 -> 1 258).
 template <int D>
-constexpr int kFaPolyEveryFor = D == 64 ? 4 : 0;
+constexpr int kFaPolyEveryFor = D == 64 ? 5 : 0;
 
 // 32 scores of one row (keys cb0 .. cb0 + 31): adds the exponentials 2^(s * sl2 - ms) of the
 // (masked) scores to the packed sums and packs them to fp16, keys (2i, 2i + 1) in pk[i].
 template <bool MASKED, int EVERY>
 __device__ __forceinline__ void fa_exp_chunk32(const uint32_t (&v)[32], int cb0, int row_abs, uint64_t sl2x2,
-                                               uint64_t nmsx2, const FaPolyConst &pc, uint64_t (&sum2)[2], uint32_t *pk) {
+                                               uint64_t nmsx2, const FaPolyConst &pc, uint64_t (&sum2)[2], float &seen,
+                                               uint32_t *pk) {
     using P16 = Pack16<DECA_F16>;
+    constexpr int kEvery = EVERY > 0 ? EVERY : 1;
+    if (!MASKED && EVERY > 0) {
+        // the saturating fma turns a NaN score into 0: the share's raw scores go into a maximum that keeps it
+#pragma unroll
+        for (int i = kEvery - 1; i < 16; i += kEvery)
+            asm("max.NaN.f32 %0, %0, %1, %2;"
+                : "+f"(seen)
+                : "f"(__uint_as_float(v[2 * i])), "f"(__uint_as_float(v[2 * i + 1])));
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         float s0 = __uint_as_float(v[2 * i]), s1 = __uint_as_float(v[2 * i + 1]);
@@ -143,7 +155,7 @@ __device__ __forceinline__ void fa_exp_chunk32(const uint32_t (&v)[32], int cb0,
             if (cb0 + 2 * i + 1 > row_abs) s1 = kNegInf;
         }
         float p0, p1;
-        if (!MASKED && EVERY > 0 && i % (EVERY > 0 ? EVERY : 1) == (EVERY > 0 ? EVERY : 1) - 1) {
+        if (!MASKED && EVERY > 0 && i % kEvery == kEvery - 1) {
             fa_exp2_poly_pair(s0, s1, pc, p0, p1);
         } else {
             float x0, x1;
@@ -167,6 +179,7 @@ __device__ __forceinline__ float fa_exp_tile_hold(uint32_t tS, int col0, int row
     const uint64_t sl2x2 = f32x2_pack(sl2, sl2), nmsx2 = f32x2_pack(-ms, -ms);
     const FaPolyConst pc = fa_poly_const(sl2, ms);
     uint64_t sum2[2] = {0ull, 0ull};
+    float seen = 0.f;  // NaN where the polynomial share has met one
     uint32_t v[2][32];
     tmem_ld_32x32b_x32(tS, v[0]);
     tmem_ld_wait_regs(v[0]);
@@ -174,14 +187,14 @@ __device__ __forceinline__ float fa_exp_tile_hold(uint32_t tS, int col0, int row
     for (int c = 0; c < kChunks; ++c) {
         if (c + 1 < kChunks) tmem_ld_32x32b_x32(tS + (c + 1) * 32, v[(c + 1) & 1]);
         // chunk c = keys 32c ..: half h = c / 2 of the tile, words (c % 2) * 16 .. of that half
-        fa_exp_chunk32<MASKED, EVERY>(v[c & 1], col0 + c * 32, row_abs, sl2x2, nmsx2, pc, sum2,
+        fa_exp_chunk32<MASKED, EVERY>(v[c & 1], col0 + c * 32, row_abs, sl2x2, nmsx2, pc, sum2, seen,
                                &pk[(c / 2) * 32 + (c % 2) * 16]);
         if (c + 1 < kChunks) tmem_ld_wait_regs(v[(c + 1) & 1]);
     }
     float a0, a1, b0, b1;
     f32x2_unpack(sum2[0], a0, a1);
     f32x2_unpack(sum2[1], b0, b1);
-    return (a0 + a1) + (b0 + b1);
+    return seen == seen ? (a0 + a1) + (b0 + b1) : seen;  // the caller's vote sends the warp to the exact pass
 }
 
 // (masked) row maximum of the tile

@@ -125,3 +125,27 @@ def test_paged_key_that_is_not_finite(value, D, dtype, max_q, max_kv):
     for kv, new, base in PLACES:
         data = special_keys(kv, new, base, value, D, dtype)
         compare(run_paged(data, 64, max_q, max_kv, D**-0.5), data, D**-0.5)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D,persistent", [(64, True), (128, True), (64, False)])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_dense_key_that_is_not_finite(value, D, persistent, causal):
+    from deca_b200.kernels.flash_attn_b200 import FAConfig
+    from deca_b200.operators import FlashAttention
+
+    op = FlashAttention(1, 8, 512, 512, D, causal=causal)
+    cfg = None if persistent else FAConfig(Bc=128, stages=4, q_tiles=2, p_tmem=True)
+    g = torch.Generator().manual_seed(7)
+    for base in (40, 72, 336):
+        q, k, v = (torch.randn(1, 8, 512, D, generator=g).half().cuda() for _ in range(3))
+        q[..., 5] = 1.0
+        for h in range(8):
+            k[0, h, base + h, 5] = value
+        got = op(q, k, v, cfg=cfg)
+        for h in range(8):
+            want, mag = formula(q[0, h], k[0, h], v[0, h], D**-0.5, 0 if causal else None)
+            have, nan = got[0, h].double(), torch.isnan(want)
+            assert torch.equal(torch.isnan(have), nan), f"key {base + h}"
+            bad = ((have - want).abs() > attention_bound(want, mag, q.dtype)) & ~nan
+            assert not bad.any(), f"key {base + h}: rows {bad.any(-1).nonzero().flatten().tolist()[:9]}"
