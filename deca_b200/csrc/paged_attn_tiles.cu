@@ -120,14 +120,16 @@ __device__ __forceinline__ void mask_tile(uint32_t tS, int visible) {
     tmem_st_wait();
 }
 
-// One key tile of the online softmax for this thread's row.  A row sees a prefix of the keys, so one that
-// sees nothing of a segment's first 32 keys sees nothing of it: m stays -inf, l and P zero.
+// One key tile of the online softmax for this thread's row; `sees`: the row belongs to a token and sees a key of this tile.
+// A row sees a prefix of the keys, so one that sees nothing of a segment's first 32 keys sees nothing of it: m
+// stays -inf, l and P zero.  Rows behind the request's last token hold other requests' queries or padding; they have
+// no voice in the warp's vote, or what they hold would choose the pass, and with it the rounding, of the others.
 // There is one copy of the exponentials' straight-line code: masked tiles are masked in place before it, and the
 // rare second pass is a loop.  The warps' roles share the instruction cache, and what falls out of it costs an
 // item microseconds when it ends (with a copy for each case 4 us from the last product of an item to the first
 // score of the next).
 template <int DT, int D>
-__device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, float sl2, bool first, float &m, float &l) {
+__device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, float sl2, bool first, bool sees, float &m, float &l) {
     if (first) {
         uint32_t v[32];
         tmem_ld_32x32b_x32(tS, v);
@@ -138,7 +140,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, float sl2
         // held in registers until the vote: storing P overwrites the scores that a second pass would need
         uint32_t pk[kBc / 2];
         const float sum = exp_row<DT>(tS, sl2, m == -INFINITY ? 0.f : m * sl2, pk);
-        if (!__any_sync(0xFFFFFFFFu, !(sum <= kFaSumLimit))) {
+        if (!__any_sync(0xFFFFFFFFu, sees && !(sum <= kFaSumLimit))) {
 #pragma unroll
             for (int h = 0; h < kBc / 64; ++h) {
                 uint32_t part[32];
@@ -562,7 +564,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 tc_fence_after_sync();
                 const int col0 = (w.step + j) * kBc;
                 if (col0 + kBc - 1 > lim_tile) mask_tile(tSg, lim + 1 - col0);
-                softmax_tile<DT, D>(tSg, tOg, sl2, j == 0, m, l);
+                softmax_tile<DT, D>(tSg, tOg, sl2, j == 0, lim >= col0, m, l);
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full(grp));

@@ -149,3 +149,20 @@ def test_dense_key_that_is_not_finite(value, D, persistent, causal):
             assert torch.equal(torch.isnan(have), nan), f"key {base + h}"
             bad = ((have - want).abs() > attention_bound(want, mag, q.dtype)) & ~nan
             assert not bad.any(), f"key {base + h}: rows {bad.any(-1).nonzero().flatten().tolist()[:9]}"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("fill", [math.nan, math.inf, 300.0])
+def test_rows_of_nobody_do_not_steer_their_neighbours(fill, D, dtype):
+    """The rows of Q behind the last token (a padded batch) lie in a tile with live rows: the results do not
+    depend on them, to the bit."""
+    from deca_b200.operators import PagedAttention
+
+    q, kc, vc, table, cu, kv = make_paged([600, 1500], [70, 40], 2, 2, D, 64, dtype)
+    op = PagedAttention(2, 2, 2, D, 64, 128, 1500, str(dtype).split(".")[1])
+    padded = torch.zeros(160, 2, D, dtype=dtype, device="cuda")
+    padded[:110] = q
+    want = op(padded, kc, vc, table, i32(cu), i32(kv))[:110].clone()
+    padded[110:] = fill
+    assert torch.equal(op(padded, kc, vc, table, i32(cu), i32(kv))[:110], want)
