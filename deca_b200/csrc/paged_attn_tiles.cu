@@ -124,6 +124,8 @@ __device__ __forceinline__ void mask_tile(uint32_t tS, int visible) {
 // A row sees a prefix of the keys, so one that sees nothing of a segment's first 32 keys sees nothing of it: m
 // stays -inf, l and P zero.  Rows behind the request's last token hold other requests' queries or padding; they have
 // no voice in the warp's vote, or what they hold would choose the pass, and with it the rounding, of the others.
+// A row that sees keys while its maximum is still -inf (all its scores so far were) has no base to take exponentials
+// against: its fast sum comes out infinite or NaN, and the second pass finds the maximum.
 // There is one copy of the exponentials' straight-line code: masked tiles are masked in place before it, and the
 // rare second pass is a loop.  The warps' roles share the instruction cache, and what falls out of it costs an
 // item microseconds when it ends (with a copy for each case 4 us from the last product of an item to the first
@@ -139,7 +141,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, float sl2
     {
         // held in registers until the vote: storing P overwrites the scores that a second pass would need
         uint32_t pk[kBc / 2];
-        const float sum = exp_row<DT>(tS, sl2, m == -INFINITY ? 0.f : m * sl2, pk);
+        const float sum = exp_row<DT>(tS, sl2, sees ? m * sl2 : 0.f, pk);
         if (!__any_sync(0xFFFFFFFFu, sees && !(sum <= kFaSumLimit))) {
 #pragma unroll
             for (int h = 0; h < kBc / 64; ++h) {

@@ -166,3 +166,24 @@ def test_rows_of_nobody_do_not_steer_their_neighbours(fill, D, dtype):
     want = op(padded, kc, vc, table, i32(cu), i32(kv))[:110].clone()
     padded[110:] = fill
     assert torch.equal(op(padded, kc, vc, table, i32(cu), i32(kv))[:110], want)
+
+
+@pytest.mark.parametrize("max_q,max_kv", SCHEDULES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dead", [32, 40, 128, 200])
+def test_paged_first_scores_minus_infinity(dead, D, dtype, max_q, max_kv):
+    """The first `dead` visible keys score -inf and the others -200 and -199: the maximum starts at -inf there and
+    the weights of the others are still theirs."""
+    for kv, new in ((400, 40), (3000, 24)):
+        data = make_paged([kv], [new], 2, 1, D, 64, dtype, seed=dead)
+        q, kc, vc, table, _, _ = data
+        q.fill_(8.0)
+        kc.fill_(-200 / 64)
+        for at in range(kv):
+            if at < dead:
+                set_key(kc, table, 0, at, 0.0, 64)
+                set_key(kc, table, 0, at, -math.inf, 64, 5)
+            elif at % 3 == 0:
+                set_key(kc, table, 0, at, -199 / 64, 64)
+        compare(run_paged(data, 64, max_q, max_kv, 8.0 / D), data, 8.0 / D)
