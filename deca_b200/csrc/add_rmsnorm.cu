@@ -18,6 +18,7 @@
 // launch latency; there a warp takes one span instead of two (256 x 8192 3.9 us), which is what shortens the chain of
 // loads.
 #include "common.cuh"
+#include "overlap.cuh"
 #include "ptx.cuh"
 
 namespace deca {
@@ -449,6 +450,20 @@ extern "C" int deca_add_rmsnorm(int dtype, const void *X, int64_t x_stride, cons
     if (!aligned_to(X, 2) || !aligned_to(R, 2) || !aligned_to(W, 2) || !aligned_to(H, 2) || !aligned_to(Y, out_bytes) ||
         !aligned_to(scales, 4))
         return DECA_ERR_ALIGN;
+    // Every element is read and written by one thread, which has read it from X and R before it writes H and Y: H and Y may
+    // each replace one of them.  W and the scales are shared between threads.
+    {
+        const Region x = region(X, 2 * N, M, 2 * x_stride), r = region(R, 2 * N, M, 2 * r_stride), w = region(W, 2 * N);
+        const Region h = region(H, 2 * N, M, 2 * h_stride), y = region(Y, out_bytes * N, M, out_bytes * y_stride);
+        const Region s = region(scales, 4, out == DECA_OUT_E4M3 ? M * (group ? (N + group - 1) / group : 1) : 0, 4);
+        for (const Region &in : {x, r}) {
+            if (!regions_equal(h, in) && !regions_apart(h, in)) return DECA_ERR_UNSUPPORTED;
+            if (!regions_equal(y, in) && !regions_apart(y, in)) return DECA_ERR_UNSUPPORTED;
+        }
+        if (!regions_apart(h, y) || !regions_apart(h, w) || !regions_apart(y, w)) return DECA_ERR_UNSUPPORTED;
+        for (const Region &other : {x, r, w, h, y})
+            if (!regions_apart(s, other)) return DECA_ERR_UNSUPPORTED;
+    }
     // elements per access: the widest that the row length, the strides and the bases allow
     int v = 8;
     auto fits = [&](int w) {

@@ -57,7 +57,8 @@ class AddRMSNorm(Operator):
 
     def __call__(self, x, res, w, out=None, res_out=None, scales=None):
         """Runs the kernel; returns (y, h), or (q, scales, h) with ``out="e4m3"``.  ``res_out`` may be ``res``
-        or ``x`` (updated in place), ``out`` may be ``x`` where it is 16 bits wide."""
+        or ``x`` (updated in place), ``out`` the other of them where it is 16 bits wide; an output that shares memory with
+        another tensor of the call in any other way is refused."""
         if self._mod is None:
             self._mod = self.compile(self.build_mod())["main"]
         if self.out == "same":

@@ -32,7 +32,7 @@ extern "C" {
 #define DECA_ERR_SHAPE (-2)       /* non-positive or unsupported extent */
 #define DECA_ERR_ALIGN (-3)       /* pointer or row pitch not aligned for the vector width / TMA */
 #define DECA_ERR_CONFIG (-4)      /* config rejected by the check_config rules */
-#define DECA_ERR_UNSUPPORTED (-5) /* op / dtype / mode not built */
+#define DECA_ERR_UNSUPPORTED (-5) /* op / dtype / mode not built; serving operators: an output over another buffer of the call */
 #define DECA_ERR_SCRATCH_LIMIT (-6) /* the problem needs more scratch memory than the built-in buffer holds */
 #define DECA_ERR_DEVICE_TIMEOUT 100001 /* a kernel's bounded wait ran out (see deca_last_device_status) */
 
@@ -263,8 +263,8 @@ int deca_fa_fwd_f16_gather(const void *Q, const void *K, const void *V, void *co
  *   A scale below the smallest normal fp32 number (all of the group's y zero, in practice) gives zeros.
  *   A NaN in a group makes its scale NaN.
  * Row strides in elements, at least N; W contiguous.  Any N: rows that are no multiple of 8 elements
- * or not 16-byte aligned take element-wise accesses.  H may be X or R itself, Y (of DECA_OUT_SAME) may
- * be X; other overlaps are not allowed.  M = 0 launches nothing.
+ * or not 16-byte aligned take element-wise accesses.  H and Y (of DECA_OUT_SAME) may each be X or R itself (same
+ * pointer and stride); other overlaps of an output are refused (DECA_ERR_UNSUPPORTED).  M = 0 launches nothing.
  * No counterpart in the reference, whose RMSNorm has neither residual nor 8-bit output.
  * ------------------------------------------------------------------------------------- */
 enum { DECA_OUT_SAME = 0, DECA_OUT_E4M3 = 1 };

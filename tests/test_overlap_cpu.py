@@ -1,0 +1,54 @@
+"""Outputs over other buffers of a call: refused by the C entries before anything is launched (no GPU is needed), apart from
+the places that are documented; regions whose columns alternate are apart.
+
+Addresses are numbers that nothing follows: a call that is not refused ends at the launch, for want of a device, with
+another code."""
+
+import ctypes
+
+import pytest
+
+OVERLAP = -5
+
+
+@pytest.fixture(scope="module")
+def native():
+    import torch
+
+    from deca_b200 import build, native as n
+
+    if torch.cuda.is_available():
+        pytest.skip("the addresses of these calls are made up: on a GPU the accepted ones would run")
+    build.build()
+    n.lib()
+    return n
+
+
+K = 1 << 20  # distance of buffers that have nothing to do with each other
+
+
+def norm(native, **kw):
+    a = {**dict(dtype=0, x=K, xs=64, r=2 * K, rs=64, w=3 * K, h=4 * K, hs=64, y=5 * K, ys=64, s=None, M=8, N=64, eps=1e-6, out=0, group=0), **kw}
+    return native.lib().deca_add_rmsnorm(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw", [
+    {"h": K}, {"h": 2 * K}, {"y": K}, {"y": 2 * K}, {"h": K, "y": 2 * K}, {"h": 2 * K, "y": K},  # in place
+    {"r": K},  # inputs may be one
+    {"h": K + 128 * 8}, {"y": K - 128 * 8},  # side by side
+    {"xs": 256, "hs": 256, "h": K + 128}, {"xs": 256, "rs": 256, "hs": 256, "ys": 256, "r": K + 128, "h": K + 256, "y": K + 384},  # columns of one buffer
+    {"h": K, "M": 1, "xs": 64, "hs": 640},  # one row: its stride is no matter
+    {"out": 1, "s": 6 * K}, {"out": 1, "s": 6 * K, "group": 32, "h": K}, {"out": 1, "s": K + 128 * 8}])
+def test_add_rmsnorm_takes(native, kw):
+    assert norm(native, **kw) not in (0, OVERLAP)
+
+
+@pytest.mark.parametrize("kw", [
+    {"h": 5 * K}, {"h": K, "y": K}, {"y": 4 * K + 128 * 7},  # h lost under y
+    {"h": 3 * K}, {"y": 3 * K + 64}, {"w": 4 * K + 1022},
+    {"h": K + 2}, {"h": K + 128}, {"y": 2 * K - 2}, {"h": K, "hs": 65}, {"h": K, "hs": 128},  # shifted, or at other strides
+    {"xs": 96, "hs": 96, "h": K + 128},  # columns that meet
+    {"out": 1, "s": K}, {"out": 1, "s": 4 * K + 4}, {"out": 1, "s": 5 * K}, {"out": 1, "s": 3 * K, "group": 32},
+    {"out": 1, "s": 6 * K, "y": K}, {"out": 1, "s": 6 * K, "y": K + 64}])
+def test_add_rmsnorm_refuses(native, kw):
+    assert norm(native, **kw) == OVERLAP

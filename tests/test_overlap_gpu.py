@@ -1,0 +1,45 @@
+"""Outputs over other tensors of a call, through the operators: in place where that is documented, with the same bits as
+tensors of their own, and refused elsewhere."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from serving_util import i32, make_paged  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("M,N", [(6, 1000), (6, 1001), (300, 513), (5, 40000), (5, 40001)])
+def test_add_rmsnorm_over_its_inputs(M, N):
+    from deca_b200.operators import AddRMSNorm
+
+    g = torch.Generator().manual_seed(N)
+    x, res = (torch.randn(M, N, generator=g).bfloat16().cuda() for _ in range(2))
+    w = torch.randn(N, generator=g).bfloat16().cuda()
+    op = AddRMSNorm(M, N, "bfloat16")
+    y, h = op(x, res, w)
+    for y_over, h_over in ((0, None), (1, None), (None, 0), (None, 1), (0, 1), (1, 0)):
+        both = [x.clone(), res.clone()]
+        got_y, got_h = op(*both, w, out=None if y_over is None else both[y_over], res_out=None if h_over is None else both[h_over])
+        assert torch.equal(got_y, y) and torch.equal(got_h, h)
+    wide = torch.cat([x, res, x, res], 1)  # columns of one buffer
+    a, b, c, d = (wide[:, i * N : (i + 1) * N] for i in range(4))
+    op(a, b, w, out=c, res_out=d)
+    assert torch.equal(c, y) and torch.equal(d, h) and torch.equal(a, x) and torch.equal(b, res)
+
+
+def test_add_rmsnorm_refuses_overlaps():
+    from deca_b200.operators import AddRMSNorm
+
+    big = torch.randn(20, 64, device="cuda").half()
+    x, res, w = big[:8], big[8:16], big[16]
+    before = big.clone()
+    op, eight = AddRMSNorm(8, 64), AddRMSNorm(8, 64, out="e4m3")
+    for call in (lambda: op(x, res, w, out=x, res_out=x), lambda: op(x, res, w, out=big[1:9]), lambda: op(x, res, w, res_out=big[4:12]),
+                 lambda: op(x, res, w, out=big[10:18]), lambda: eight(x, res, w, out=x.view(torch.float8_e4m3fn)[:, :64]),
+                 lambda: eight(x, res, w, scales=res.view(torch.float32).view(-1)[:8].view(8, 1))):
+        with pytest.raises(RuntimeError, match="another buffer"):
+            call()
+    torch.cuda.synchronize()
+    assert torch.equal(big, before)
