@@ -12,6 +12,7 @@
 // rate; 4099 tokens of 24 heads 10.6 us; 8 tokens 2.7 us (launch latency; a token's heads are then shared by several
 // CTAs).  A CTA per token without the walk took 40 us, with one unit in flight per thread instead of three 53.
 #include "common.cuh"
+#include "overlap.cuh"
 #include "ptx.cuh"
 
 namespace deca {
@@ -205,6 +206,10 @@ bool vector_ok(const deca_cache *c) {
     return aligned_to(c->data, 16) && c->page_stride % 8 == 0 && c->row_stride % 8 == 0 && c->head_stride % 8 == 0;
 }
 
+Region region_of(const deca_tokens *t, int64_t tokens, int heads, int D) {
+    return region(t->data, 2 * (int64_t)D, tokens, 2 * t->token_stride, heads, 2 * t->head_stride);
+}
+
 template <int DT, int V>
 void launch_layout(const RotArgs &g, const Turns &t, int layout, dim3 grid, unsigned threads, cudaStream_t st) {
     if (layout == DECA_ROT_HALF)
@@ -259,6 +264,9 @@ extern "C" int deca_rotary(int dtype, const deca_tokens *X, const deca_tokens *Y
     if (tokens == 0) return DECA_OK;
     if (!X->data || !Y->data || !positions) return DECA_ERR_NULL;
     if (!aligned_to(X->data, 2) || !aligned_to(Y->data, 2) || !aligned_to(positions, 4)) return DECA_ERR_ALIGN;
+    // a pair is read and written by one thread, so Y may be X
+    const Region x = region_of(X, tokens, heads, rot->D), y = region_of(Y, tokens, heads, rot->D);
+    if ((!regions_equal(x, y) && !regions_apart(x, y)) || !regions_apart(y, region(positions, 4 * tokens))) return DECA_ERR_UNSUPPORTED;
     RotArgs g = {};
     g.q = static_cast<const char *>(X->data), g.q_st = X->token_stride, g.q_sh = X->head_stride;
     g.qo = static_cast<char *>(Y->data), g.qo_st = Y->token_stride, g.qo_sh = Y->head_stride;

@@ -48,7 +48,8 @@ class Rotary(Operator):
         return rotary_frequencies(self.rot_dim, self.base, self.scaling)
 
     def __call__(self, x, positions, out=None, inverse: bool = False):
-        """Returns x [T, H, D] turned by ``positions`` [T] (int32); ``out`` may be ``x``."""
+        """Returns x [T, H, D] turned by ``positions`` [T] (int32); ``out`` may be ``x``, and is refused where it shares
+        memory with x or the positions in any other way."""
         if self._mod is None:
             self._mod = self.compile(self.build_mod())["main"]
         return self._mod(x, positions, out, inverse)

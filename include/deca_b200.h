@@ -301,7 +301,8 @@ typedef struct {
     const uint64_t *turns; /* host array, rot_dim / 2 entries */
 } deca_rotation;
 
-/* Y[t, h] = rotate(X[t, h], positions[t]); Y may be X itself (same pointer and strides). */
+/* Y[t, h] = rotate(X[t, h], positions[t]); Y may be X itself (same pointer and strides), other overlaps of Y are
+ * refused (DECA_ERR_UNSUPPORTED). */
 int deca_rotary(int dtype, const deca_tokens *X, const deca_tokens *Y, const int32_t *positions, int64_t tokens,
                 int heads, const deca_rotation *rot, void *stream);
 

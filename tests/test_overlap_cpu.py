@@ -52,3 +52,28 @@ def test_add_rmsnorm_takes(native, kw):
     {"out": 1, "s": 6 * K, "y": K}, {"out": 1, "s": 6 * K, "y": K + 64}])
 def test_add_rmsnorm_refuses(native, kw):
     assert norm(native, **kw) == OVERLAP
+
+
+def tokens(native, at, token=128, head=64):
+    return native.Tokens(at, token, head)
+
+
+def rotation(native):
+    return native.Rotation(D=64, rot_dim=64, layout=0, inverse=0, amplitude=1.0, turns=(ctypes.c_uint64 * 32)())
+
+
+def rotary(native, x, y, pos=9 * K, T=8, H=2):
+    return native.lib().deca_rotary(0, tokens(native, *x), tokens(native, *y), pos, T, H, rotation(native), None)
+
+
+# X and Y as (address, token stride, head stride)
+@pytest.mark.parametrize("x,y", [((K,), (2 * K,)), ((K,), (K,)), ((K, 256), (K + 256, 256)), ((K, 64, 1024), (K + 128 * 8, 64, 1024)),
+                                 ((K, 192, 64), (K, 192, 64)), ((K, 0, 0), (2 * K,)), ((K, 256, 128), (K + 128, 256, 128))])
+def test_rotary_takes(native, x, y):
+    assert rotary(native, x, y) not in (0, OVERLAP)
+
+
+@pytest.mark.parametrize("x,y,pos", [((K,), (K + 16,), 9 * K), ((K,), (K + 128,), 9 * K), ((K,), (K, 64, 512), 9 * K), ((K, 192), (K + 128, 192), 9 * K),
+                                     ((K, 0, 0), (K,), 9 * K), ((K,), (2 * K,), 2 * K + 4), ((K,), (K - 2032,), 9 * K)])
+def test_rotary_refuses(native, x, y, pos):
+    assert rotary(native, x, y, pos) == OVERLAP

@@ -43,3 +43,23 @@ def test_add_rmsnorm_refuses_overlaps():
             call()
     torch.cuda.synchronize()
     assert torch.equal(big, before)
+
+
+def test_rotary_refuses_overlaps():
+    from deca_b200.operators import Rotary
+
+    g = torch.Generator().manual_seed(1)
+    buffer = torch.randn(20 * 6 * 64, generator=g).half().cuda()
+    before = buffer.clone()
+    x = buffer[: 12 * 4 * 64].view(12, 4, 64)
+    op, pos = Rotary(64), i32(list(range(12)))
+    for out in (buffer[64 : 64 + x.numel()].view(12, 4, 64), buffer[2 : 2 + x.numel()].view(12, 4, 64), buffer.as_strided((12, 4, 64), (64, 12 * 64, 1)),
+                buffer[32 * 64 :][: x.numel()].view(12, 4, 64)):
+        with pytest.raises(RuntimeError, match="another buffer"):
+            op(x, pos, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(buffer, before)
+    halves = torch.zeros(12, 8, 64, dtype=torch.float16, device="cuda")
+    halves[:, :4] = x
+    op(halves[:, :4], pos, out=halves[:, 4:])
+    assert torch.equal(halves[:, 4:], op(x, pos)) and torch.equal(halves[:, :4], x)
