@@ -55,7 +55,7 @@ inline bool regions_apart(const Region &a, const Region &b) {
         region_span(b, pitch, &b0, &bn);
         if (pitch == 0) return a0 + an <= b0 || b0 + bn <= a0;
         if (an > pitch || bn > pitch) return false;
-        __int128 d = (b0 - a0) % pitch;
+        int64_t d = (int64_t)(b0 - a0) % pitch;
         if (d < 0) d += pitch;
         return d >= an && d + bn <= pitch;
     };

@@ -290,6 +290,21 @@ extern "C" int deca_rotary_append(int dtype, const deca_tokens *Q, const deca_to
     if (!aligned_to(positions, 4) || !aligned_to(slots, 8) || !aligned_to(Q->data, 2) || !aligned_to(K->data, 2) ||
         !aligned_to(V->data, 2) || !aligned_to(Q_out->data, 2) || !aligned_to(K_cache->data, 2) || !aligned_to(V_cache->data, 2))
         return DECA_ERR_ALIGN;
+    {
+        const int D = rot->D;
+        auto cache = [&](const deca_cache *c) {
+            return region(c->data, 2 * (int64_t)D, num_pages, 2 * c->page_stride, page_size, 2 * c->row_stride, H_kv, 2 * c->head_stride);
+        };
+        const Region q = region_of(Q, tokens, H_q, D), k = region_of(K, tokens, H_kv, D), v = region_of(V, tokens, H_kv, D);
+        const Region out = region_of(Q_out, tokens, H_q, D), kc = cache(K_cache), vc = cache(V_cache);
+        const Region pos = region(positions, 4 * tokens), slot = region(slots, 8 * tokens);
+        if (!regions_equal(q, out) && !regions_apart(q, out)) return DECA_ERR_UNSUPPORTED;
+        if (!regions_apart(out, kc) || !regions_apart(out, vc) || !regions_apart(kc, vc)) return DECA_ERR_UNSUPPORTED;
+        for (const Region &in : {k, v, pos, slot})
+            if (!regions_apart(in, out)) return DECA_ERR_UNSUPPORTED;
+        for (const Region &in : {q, k, v, pos, slot})
+            if (!regions_apart(in, kc) || !regions_apart(in, vc)) return DECA_ERR_UNSUPPORTED;
+    }
     RotArgs g = {};
     g.q = static_cast<const char *>(Q->data), g.q_st = Q->token_stride, g.q_sh = Q->head_stride;
     g.k = static_cast<const char *>(K->data), g.k_st = K->token_stride, g.k_sh = K->head_stride;

@@ -79,7 +79,8 @@ class RotaryAppend(Rotary):
 
     def __call__(self, q, k, v, positions, slots, k_cache, v_cache, out=None):
         """q [T, H_q, D], k and v [T, H_kv, D] (views of one projection will do), positions [T] int32, slots [T]
-        int64; returns the turned q (``out`` may be ``q``)."""
+        int64; returns the turned q (``out`` may be ``q``).  An output or a cache that shares memory with another tensor of
+        the call in any other way is refused; views whose elements alternate in one buffer do not share any."""
         if self._mod is None:
             self._mod = self.compile(self.build_mod())["main"]
         return self._mod(q, k, v, positions, slots, k_cache, v_cache, out)

@@ -308,7 +308,8 @@ int deca_rotary(int dtype, const deca_tokens *X, const deca_tokens *Y, const int
 
 /* Q_out = rotate(Q); row slots[t] of the cache = rotate(K[t]), V[t] in one launch, where slot s is row
  * s % page_size of page s / page_size.  A slot outside [0, num_pages * page_size) writes nothing (padding
- * rows carry -1); two tokens must not share a slot.  Q_out may be Q itself. */
+ * rows carry -1); two tokens must not share a slot.  Q_out may be Q itself; other overlaps of Q_out and the caches with
+ * each other or with an input are refused (DECA_ERR_UNSUPPORTED). */
 int deca_rotary_append(int dtype, const deca_tokens *Q, const deca_tokens *K, const deca_tokens *V,
                        const deca_tokens *Q_out, const deca_cache *K_cache, const deca_cache *V_cache,
                        const int32_t *positions, const int64_t *slots, int64_t tokens, int H_q, int H_kv,

@@ -77,3 +77,38 @@ def test_rotary_takes(native, x, y):
                                      ((K, 0, 0), (K,), 9 * K), ((K,), (2 * K,), 2 * K + 4), ((K,), (K - 2032,), 9 * K)])
 def test_rotary_refuses(native, x, y, pos):
     assert rotary(native, x, y, pos) == OVERLAP
+
+
+def cache(native, at, page=2048, row=128, head=64):
+    return native.Cache(at, page, row, head)
+
+
+def append(native, **kw):
+    """8 tokens of 4 + 2 x 2 heads of 64 into 3 pages of 16 rows."""
+    a = {**dict(q=(K, 256), k=(2 * K,), v=(3 * K,), out=(4 * K, 256), kc=(5 * K,), vc=(6 * K,), pos=7 * K, slots=8 * K, pages=3), **kw}
+    q, k, v, out = (tokens(native, *a[n]) for n in ("q", "k", "v", "out"))
+    return native.lib().deca_rotary_append(0, q, k, v, out, cache(native, *a["kc"]), cache(native, *a["vc"]), a["pos"], a["slots"], 8, 4, 2,
+                                           a["pages"], 16, rotation(native), None)
+
+
+PROJECTION = {"q": (K, 512), "k": (K + 512, 512), "v": (K + 768, 512)}  # column blocks of one buffer
+
+
+@pytest.mark.parametrize("kw", [
+    {}, {"out": (K, 256)}, PROJECTION, {**PROJECTION, "out": (K, 512)}, {"k": (2 * K, 0, 0), "v": (2 * K, 0, 0)},
+    {"kc": (5 * K, 4096), "vc": (5 * K + 4096, 4096)},  # pages of keys, then values
+    {"kc": (5 * K, 4096, 256), "vc": (5 * K + 256, 4096, 256)},  # rows of keys, then values
+    {"kc": (5 * K, 4096, 256, 128), "vc": (5 * K + 128, 4096, 256, 128)},  # heads of keys, then values
+    {"kc": (5 * K, 4096, 64, 1024), "vc": (5 * K + 4096, 4096, 64, 1024)},  # head by head
+    {"kc": (5 * K,), "vc": (5 * K + 3 * 4096,)}, {"kc": (5 * K, 1, 128), "vc": (5 * K + 4096, 7, 128), "pages": 1}])
+def test_rotary_append_takes(native, kw):
+    assert append(native, **kw) not in (0, OVERLAP)
+
+
+@pytest.mark.parametrize("kw", [
+    {**PROJECTION, "out": (K + 512, 512)}, {**PROJECTION, "out": (K + 128, 512)}, {"out": (K + 128, 256)}, {"out": (2 * K, 256)}, {"out": (3 * K - 128, 256)},
+    {"kc": (6 * K,)}, {"kc": (6 * K + 128,)}, {"kc": (5 * K, 4096), "vc": (5 * K + 2048, 4096)}, {"kc": (5 * K, 4096, 256), "vc": (5 * K + 128, 4096, 256)},
+    {"out": (5 * K, 256)}, {"out": (6 * K + 4096, 256)}, {"q": (5 * K, 256)}, {"k": (5 * K + 3 * 4096 - 2,)}, {"v": (6 * K,)}, {"k": (6 * K,)},
+    {"pos": 5 * K}, {"slots": 6 * K + 16}, {"pos": 4 * K + 4}, {"slots": 4 * K + 2040}])
+def test_rotary_append_refuses(native, kw):
+    assert append(native, **kw) == OVERLAP

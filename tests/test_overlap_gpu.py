@@ -63,3 +63,26 @@ def test_rotary_refuses_overlaps():
     halves[:, :4] = x
     op(halves[:, :4], pos, out=halves[:, 4:])
     assert torch.equal(halves[:, 4:], op(x, pos)) and torch.equal(halves[:, :4], x)
+
+
+def test_rotary_append_refuses_overlaps():
+    from deca_b200.operators import RotaryAppend
+
+    g = torch.Generator().manual_seed(2)
+    T, Hq, Hkv, D, page = 9, 4, 2, 64, 16
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * D, generator=g).half().cuda()
+    q, k, v = (t.view(T, -1, D) for t in qkv.split([Hq * D, Hkv * D, Hkv * D], -1))
+    both = torch.zeros(3, page, 2, Hkv, D, dtype=torch.float16, device="cuda")  # rows of keys, then values
+    kc, vc = both[:, :, 0], both[:, :, 1]
+    before, slots, pos = qkv.clone(), torch.arange(T, device="cuda"), i32(list(range(T)))
+    op = RotaryAppend(Hq, Hkv, D, page)
+    for out, caches in ((qkv[:, 2 * D : 6 * D].view(T, 4, D), (kc, vc)), (both.view(-1)[: T * Hq * D].view(T, Hq, D), (kc, vc)), (None, (kc, kc)),
+                        (None, (both.view(3, 2, page, Hkv, D)[:, 0], vc))):
+        with pytest.raises(RuntimeError, match="another buffer"):
+            op(q, k, v, pos, slots, *caches, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(qkv, before) and not both.any()
+    want_k, want_v = torch.zeros(2, 3, page, Hkv, D, dtype=torch.float16, device="cuda")
+    want = op(q, k, v, pos, slots, want_k, want_v)
+    assert op(q, k, v, pos, slots, kc, vc, out=q) is not None
+    assert torch.equal(q, want) and torch.equal(kc, want_k) and torch.equal(vc, want_v) and torch.equal(v, before[:, 6 * D :].view(T, Hkv, D))
