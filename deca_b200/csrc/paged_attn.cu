@@ -1,6 +1,7 @@
 // Entry points of the paged attention: argument rules, choice of the schedule, workspace.
 #include <cmath>
 
+#include "overlap.cuh"
 #include "paged_attn.cuh"
 
 namespace deca {
@@ -68,6 +69,21 @@ bool query_strides(const deca_paged_attn_args &a, long long &st, long long &sh) 
     return ok;
 }
 
+// O may replace Q (an item's rows are read before the same rows are written) and must be apart from all else; the
+// workspace from everything.
+bool outputs_apart(const deca_paged_attn_args &a) {
+    auto tokens = [&](const deca_tokens &t) { return region(t.data, 2 * a.D, a.T, 2 * t.token_stride, a.H_q, 2 * t.head_stride); };
+    auto cache = [&](const deca_cache &c) {
+        return region(c.data, 2 * a.D, a.num_pages, 2 * c.page_stride, a.page_size, 2 * c.row_stride, a.H_kv, 2 * c.head_stride);
+    };
+    const Region q = tokens(a.Q), o = tokens(a.O), ws = region(a.workspace, (int64_t)a.workspace_bytes);
+    if (!regions_equal(q, o) && !regions_apart(q, o)) return false;
+    for (const Region &r : {cache(a.K), cache(a.V), region(a.block_table, 4ll * a.table_width, a.B, 4 * a.table_stride), region(a.cu_q, 4 * (a.B + 1ll)),
+                            region(a.kv_lens, 4ll * a.B)})
+        if (!regions_apart(r, o) || !regions_apart(r, ws)) return false;
+    return regions_apart(q, ws) && regions_apart(o, ws);
+}
+
 }  // namespace
 }  // namespace deca
 
@@ -107,6 +123,7 @@ extern "C" int deca_paged_attn_workspace_bytes(const deca_paged_attn_args *a, si
 extern "C" int deca_paged_attn(const deca_paged_attn_args *a, void *stream) {
     if (int rc = deca_paged_attn_check(a)) return rc;
     if (a->T == 0) return DECA_OK;
+    if (!outputs_apart(*a)) return DECA_ERR_UNSUPPORTED;
     size_t need = 0;
     if (int rc = deca_paged_attn_workspace_bytes(a, &need)) return rc;
     if (need > 0 && !a->workspace) return DECA_ERR_NULL;

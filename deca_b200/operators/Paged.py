@@ -114,7 +114,8 @@ class PagedAttention(Operator):
     def __call__(self, q, k_cache, v_cache, block_table, cu_q, kv_lens, out=None):
         """q [T, H_q, D]: request r owns rows cu_q[r] .. cu_q[r + 1] - 1; caches [pages, page_size, H_kv, D];
         block_table [B, width], cu_q [B + 1], kv_lens [B], int32 on the device.  Returns O [T, H_q, D] (``out`` may
-        be ``q``).  Rows that belong to no request are not written.
+        be ``q``, and is refused where it shares memory with a tensor of the call in any other way).  Rows that belong to no
+        request are not written.
 
         Lengths are clipped to what q and the table hold, a table entry that names no page reads as zeros, and
         what a token does not see does not reach its output, whatever the cache holds there."""

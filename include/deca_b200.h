@@ -345,8 +345,9 @@ int deca_paged_step(const int32_t *ctx_lens, const int32_t *new_lens, int B, int
  * Lengths are read on the device and clipped to what T and the table hold; a table entry that names no
  * page reads as zeros.  What a row cannot see never reaches it, whatever the cache holds there.
  * max_q / max_kv: upper bounds of a request's new tokens and cached length as the caller knows them;
- * they choose the schedule (any values give right results).  O may be Q; strides of Q, K and V are positive
- * (K and V may have a head stride of 0: one key head seen as several).
+ * they choose the schedule (any values give right results).  O may be Q (same pointer and strides); other overlaps of O
+ * or the workspace with a buffer of the call are refused (DECA_ERR_UNSUPPORTED; _check leaves them to the launch).
+ * Strides of Q, K and V are positive (K and V may have a head stride of 0: one key head seen as several).
  * ------------------------------------------------------------------------------------- */
 typedef struct {
     int dtype;

@@ -112,3 +112,30 @@ def test_rotary_append_takes(native, kw):
     {"pos": 5 * K}, {"slots": 6 * K + 16}, {"pos": 4 * K + 4}, {"slots": 4 * K + 2040}])
 def test_rotary_append_refuses(native, kw):
     assert append(native, **kw) == OVERLAP
+
+
+def attend(native, **kw):
+    a = native.PagedAttnArgs(dtype=0, B=2, H_q=4, H_kv=2, D=64, page_size=16, causal=1, scale=0.125, T=8, num_pages=3, table_stride=5,
+                             table_width=5, max_q=2, max_kv=70, Q=tokens(native, K, 256), O=tokens(native, 2 * K, 256),
+                             K=cache(native, 3 * K), V=cache(native, 4 * K), block_table=5 * K, cu_q=6 * K, kv_lens=7 * K,
+                             workspace=8 * K, workspace_bytes=1 << 16)
+    for name, v in kw.items():
+        setattr(a, name, {"Q": tokens, "O": tokens, "K": cache, "V": cache}[name](native, *v) if isinstance(v, tuple) else v)
+    assert native.lib().deca_paged_attn_check(ctypes.byref(a)) == 0
+    return native.lib().deca_paged_attn(ctypes.byref(a), None)
+
+
+@pytest.mark.parametrize("kw", [
+    {}, {"O": (K, 256)}, {"Q": (K, 512), "O": (K, 512)}, {"Q": (K, 512), "O": (K + 512, 512)}, {"Q": (K, 512, 128), "O": (K + 128, 512, 128)},
+    {"V": (3 * K,)}, {"V": (3 * K + 128, 4096, 256, 128), "K": (3 * K, 4096, 256, 128)}, {"K": (3 * K, 1024, 64, 0)},
+    {"Q": (K, 64, 512), "O": (K, 64, 512)}, {"O": (K + 4096, 256)}])
+def test_paged_attention_takes(native, kw):
+    assert attend(native, **kw) not in (0, OVERLAP)
+
+
+@pytest.mark.parametrize("kw", [
+    {"O": (K + 128, 256)}, {"O": (K + 16, 256)}, {"O": (K, 512)}, {"O": (K, 64, 512)}, {"Q": (K, 512), "O": (K + 256, 512)},
+    {"O": (3 * K, 256)}, {"O": (4 * K + 3 * 4096 - 128, 256)}, {"block_table": 2 * K + 64}, {"cu_q": 2 * K + 4000}, {"kv_lens": 2 * K},
+    {"workspace": K}, {"workspace": 2 * K}, {"workspace": 3 * K + 4096}, {"workspace": 4 * K}, {"workspace": 5 * K}, {"workspace": 6 * K}, {"workspace": 7 * K - 256}])
+def test_paged_attention_refuses(native, kw):
+    assert attend(native, **kw) == OVERLAP

@@ -86,3 +86,26 @@ def test_rotary_append_refuses_overlaps():
     want = op(q, k, v, pos, slots, want_k, want_v)
     assert op(q, k, v, pos, slots, kc, vc, out=q) is not None
     assert torch.equal(q, want) and torch.equal(kc, want_k) and torch.equal(vc, want_v) and torch.equal(v, before[:, 6 * D :].view(T, Hkv, D))
+
+
+@pytest.mark.parametrize("max_q", [1, 1000])
+def test_paged_attention_refuses_overlaps(max_q):
+    from deca_b200.operators import PagedAttention
+
+    q, kc, vc, table, cu, kv = make_paged([300, 70], [40, 1], 8, 2, 64, 32, torch.bfloat16, fill=0.0)
+    buffer = torch.zeros(50 * 8 * 64, dtype=q.dtype, device="cuda")
+    inside = buffer[: q.numel()].view(q.shape)
+    inside.copy_(q)
+    before, k_before = buffer.clone(), kc.clone()
+    op = PagedAttention(2, 8, 2, 64, 32, max_q, 300, "bfloat16")
+    for out in (buffer[512 : 512 + q.numel()].view(q.shape), buffer[8 : 8 + q.numel()].view(q.shape), kc.view(-1)[: q.numel()].view(q.shape),
+                buffer.as_strided(q.shape, (64, 41 * 64, 1))):
+        with pytest.raises(RuntimeError, match="another buffer"):
+            op(inside, kc, vc, table, i32(cu), i32(kv), out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(buffer, before) and torch.equal(kc, k_before)
+    want = op(q, kc, vc, table, i32(cu), i32(kv))
+    wide = torch.zeros(41, 16, 64, dtype=q.dtype, device="cuda")  # heads of q, then of the output
+    wide[:, :8] = q
+    op(wide[:, :8], kc, vc, table, i32(cu), i32(kv), out=wide[:, 8:])
+    assert torch.equal(wide[:, 8:], want) and torch.equal(wide[:, :8], q)
