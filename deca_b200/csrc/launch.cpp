@@ -57,8 +57,8 @@ std::string text_of(at::IntArrayRef v) {
 }
 
 // A CUDA tensor on the current device with this type and shape whose last dimension is contiguous.  Kernels are
-// launched on the current device's current stream and record no gradient, so what lives elsewhere or
-// asks for one is refused.
+// launched on the current device's current stream and record no gradient, so what lives elsewhere, asks for
+// one or carries a tangent is refused.
 const at::Tensor &view(PyObject *o, const char *name, at::ScalarType dtype, at::IntArrayRef shape, int device) {
     if (!THPVariable_Check(o)) {
         PyErr_Format(PyExc_TypeError, "%s: expected a tensor, got %s", name, Py_TYPE(o)->tp_name);
@@ -77,6 +77,7 @@ const at::Tensor &view(PyObject *o, const char *name, at::ScalarType dtype, at::
         refuse(std::string(name) + ": on cuda:" + std::to_string(t.get_device()) + ", but the current device is cuda:" + std::to_string(device));
     if (t.requires_grad() && c10::GradMode::is_enabled())
         refuse(std::string(name) + ": requires grad, but this operator records no gradient; call it under torch.no_grad()");
+    if (t._fw_grad(0).defined()) refuse(std::string(name) + ": carries a forward-mode tangent, but this operator computes none");
     return t;
 }
 
