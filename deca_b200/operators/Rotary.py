@@ -19,7 +19,8 @@ class Rotary(Operator):
                  scaling: dict | None = None, dtype: str = "float16", name: str = "Rotary"):
         from ..kernels.rowwise_bench import canonical_dtype
 
-        self.D, self.rot_dim, self.base, self.layout, self.scaling = D, rot_dim or D, base, layout, scaling
+        self.D, self.rot_dim = D, D if rot_dim is None else rot_dim
+        self.base, self.layout, self.scaling = base, layout, scaling
         self.dtype = canonical_dtype(dtype)
         self._mod = None
         super().__init__(name=name)
