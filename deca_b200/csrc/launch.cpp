@@ -77,6 +77,7 @@ const at::Tensor &view(PyObject *o, const char *name, at::ScalarType dtype, at::
         refuse(std::string(name) + ": on cuda:" + std::to_string(t.get_device()) + ", but the current device is cuda:" + std::to_string(device));
     if (t.requires_grad() && c10::GradMode::is_enabled())
         refuse(std::string(name) + ": requires grad, but this operator records no gradient; call it under torch.no_grad()");
+    if (t.is_neg()) refuse(std::string(name) + ": a view with pending negation; call it on tensor.resolve_neg()");
     if (t._fw_grad(0).defined()) refuse(std::string(name) + ": carries a forward-mode tangent, but this operator computes none");
     return t;
 }

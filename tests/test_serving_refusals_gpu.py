@@ -32,3 +32,18 @@ def test_forward_mode_tangents_are_refused():
             op(dq, kc, vc, table, i32(cu), i32(kv))
         op(fwd.unpack_dual(dq).primal, kc, vc, table, i32(cu), i32(kv))
     torch.cuda.synchronize()
+
+
+def test_pending_negation_is_refused():
+    """The imaginary part of a conjugated complex tensor is a view whose memory holds the values with the other sign."""
+    from deca_b200.operators import AddRMSNorm, Rotary
+
+    z = torch.complex(*torch.randn(2, 4, 64, device="cuda").half())
+    x = torch._neg_view(z.imag.contiguous())
+    assert x.is_neg()
+    w = torch.ones(64, device="cuda").half()
+    for call in (lambda t: AddRMSNorm(4, 64)(t, w.expand(4, 64).contiguous(), w), lambda t: Rotary(64)(t[:, None], i32([0, 1, 2, 3]))):
+        with pytest.raises(ValueError, match="negation"):
+            call(x)
+        call(x.resolve_neg())
+    torch.cuda.synchronize()
