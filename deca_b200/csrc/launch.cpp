@@ -282,6 +282,7 @@ PyObject *rotary(PyObject *, PyObject *const *args, Py_ssize_t n) {
         const int dev = launch_device(args[1], "x");
         const at::Tensor &x = view(args[1], "x", dt, {ANY, ANY, p.D}, dev);
         const int64_t T = x.size(0), H = x.size(1);
+        if (H > 65536) refuse("x: more than 65536 heads");  // the entry counts them in 32 bits
         const at::Tensor &pos = view(args[2], "positions", at::kInt, {T}, dev);
         at::Tensor y = output(args, n, 3, "out", dt, {T, H, p.D}, dev);
         no_overlap(y, "out");

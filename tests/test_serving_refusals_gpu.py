@@ -47,3 +47,15 @@ def test_pending_negation_is_refused():
             call(x)
         call(x.resolve_neg())
     torch.cuda.synchronize()
+
+
+def test_more_heads_than_an_int_holds_are_refused():
+    """2^32 + 2 heads (one, expanded) are not two."""
+    from deca_b200.operators import Rotary
+
+    x = torch.ones(1, 1, 2, device="cuda").half()
+    for H in (2**32 + 2, 2**31 + 1, 65537):
+        with pytest.raises(ValueError, match="heads"):
+            Rotary(2)(x.expand(1, H, 2), i32([0]))
+    assert Rotary(2)(x.expand(1, 65536, 2), i32([0])).shape == (1, 65536, 2)
+    torch.cuda.synchronize()
