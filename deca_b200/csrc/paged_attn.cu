@@ -26,8 +26,8 @@ int row_tiles(const deca_paged_attn_args &a) { return (int64_t)a.max_q * (a.H_q 
 // The tensor-core tiles take what has more than 32 query rows per request and key head, and from 17 rows on what the
 // streaming schedule divides badly.  Measured with 17 .. 32 rows (D = 128, 8 key heads, streamed / tiles): few pairs of
 // long contexts, 8 x 4000 keys 68 / 49 us, 1 x 8192 53 / 23, 9 x 1500 46 / 36 (D = 64: 1 x 8192 34 / 19, 4 x 4000 25 /
-// 26), but 2 x 500 15.8 / 16.0; more pairs than CTAs, 64 x 2000 .. 8000 397 / 354, 100 x 0 .. 3000 202 / 170, but
-// 200 x 0 .. 2000 225 / 242 and D = 64 64 x 2000 .. 8000 191 / 265.  Between them, 32 x 3000 87 / 119.
+// 26), but 2 x 500 15.8 / 16.0; more pairs than CTAs, 64 x 2000 .. 8000 397 / 351, 100 x 0 .. 3000 202 / 170, but
+// 200 x 0 .. 2000 233 / 239 and D = 64 64 x 2000 .. 8000 189 / 253.  Between them, 32 x 3000 88 / 120.
 bool use_tiles(const deca_paged_attn_args &a, int sms) {
     const int64_t rows = (int64_t)a.max_q * (a.H_q / a.H_kv), pairs = (int64_t)a.B * a.H_kv;
     if (rows <= 16 || !(a.scale > 0.f)) return false;  // the tiles keep maxima of unscaled scores

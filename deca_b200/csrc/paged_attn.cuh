@@ -108,7 +108,7 @@ struct PackedRows {
 template <int KEYS>
 struct TokenTiles {
     static constexpr int ROWS = 256;
-    // Device time without / with 1 / 2 / 3 / 4 steps: 9 requests of 188 .. 700 tokens and up to 5000 keys (D = 64)
+    // Device time without / with 1 / 2 / 3 / 4 steps (at D = 64 with a slower exponential than today's): 9 requests of 188 .. 700 tokens and up to 5000 keys (D = 64)
     // 187 / 151 / 134 / 139 / 142 us, 20 of up to 700 tokens (D = 128) 362 / 302 / 290 / 294 / 300, one of 8192 tokens
     // 547 / 507 / 488 / 494 / 501, 4 of 4096 with equal heads 342 / 329 / 332 / 319 / 324.
     static constexpr int kItemSteps = 2;

@@ -15,11 +15,11 @@
 //     key become zero, whatever the cache holds there; an element that is not finite in a key that only
 //     some of the item's rows see is replaced by zero and noted (first such key of each column and
 //     kind), and the epilogue gives it to the rows that do see it.
-// Bound by the chain of a step (scores, exponentials, product): 3550 clocks at D = 128 and 3100 at D = 64 for 2 x 128 x
-// 128 scores, of which the softmax of a tile takes 1480 and 1340 and its MMAs 1500 and 1220 up to the next scores'
-// arrival, the two tiles' MMAs following each other.  Device time: 2 x 2048 tokens behind 6144 (fp16, D = 128, 4 query
-// heads a key head) 421 us = 1.14 PFLOPS (the dense persistent schedule: 1.09 sustained, 1.28 in isolated launches), 1 x 8192 484,
-// 4 x 4096 with 16 equal heads 330 (D = 64: 267), a ragged batch of 9 at D = 64 134.
+// Bound by the chain of a step (scores, exponentials, product): 2.2 us at D = 128 and 1.8 - 1.9 at D = 64 for 2 x 128 x 128
+// scores; of the 3550 clocks at D = 128 the softmax of a tile takes 1480 and its MMAs 1500 up to the next scores' arrival,
+// the two tiles' MMAs following each other.  Device time: 2 x 2048 tokens behind 6144 (fp16, D = 128, 4 query
+// heads a key head) 420 - 425 us = 1.14 PFLOPS (the dense persistent schedule: 1.09 sustained, 1.28 in isolated launches), 1 x 8192 485,
+// 4 x 4096 with 16 equal heads 325 (D = 64: 258), a ragged batch of 9 at D = 64 127.
 // Tried and slower: two warps per 32 rows (445 us on the first of these), an issuing thread per tile (567), P in
 // columns of its own at D = 64, which tensor memory has room for, so that scores run ahead (6 % on the last); no gain:
 // the next item's first scores issued before the last product (426).

@@ -65,7 +65,9 @@ class PagedAttention(Operator):
     ``B`` requests; ``H_q`` query heads share ``H_kv`` key heads; D = 64 or 128; page sizes 16 to 256 (powers of
     two); fp16 or bf16 with fp32 scores, statistics and accumulators.  ``max_q`` and ``max_kv`` are the caller's
     bounds on a request's new and cached tokens: they choose the schedule, any value gives right
-    results.  ``causal``: a token sees the keys up to its own place (its request's new tokens are the last of
+    results.  A capacity for ``max_kv`` costs a step of short contexts at most 3 us; a chunk's budget for ``max_q`` makes
+    a step that only decodes up to twice as slow, so keep one operator for decoding (``max_q`` 1, or the length of a guess)
+    and one for chunks.  ``causal``: a token sees the keys up to its own place (its request's new tokens are the last of
     its ``kv_lens`` keys); otherwise all of them.  A token that sees nothing gets zeros.
     """
 

@@ -341,11 +341,13 @@ int deca_paged_step(const int32_t *ctx_lens, const int32_t *new_lens, int B, int
  * O[t, h] = softmax(scale * Q[t, h] K^T) V over the keys j <= kv_len - q_len + i (i = the token's place in
  * its request; causal = 0: over all kv_len keys), key head h / (H_q / H_kv).  A row that sees no key is
  * zero.  Rows of Q and O that belong to no request are not touched.  fp16 or bf16, fp32 scores, statistics
- * and accumulators, D = 64 or 128, page_size 16, 32, 64, 128 or 256, H_q / H_kv <= 128.
+ * and accumulators; the probabilities are rounded to 16 bits for the product with V (their sum is not).  A NaN or an infinity in
+ * what a row sees reaches it as in the formula (NaN for a NaN or a score of +inf, no weight for one of -inf); a row
+ * whose scores are all -inf gives zeros.  D = 64 or 128, page_size 16, 32, 64, 128 or 256, H_q / H_kv <= 128.
  * Lengths are read on the device and clipped to what T and the table hold; a table entry that names no
  * page reads as zeros.  What a row cannot see never reaches it, whatever the cache holds there.
  * max_q / max_kv: upper bounds of a request's new tokens and cached length as the caller knows them;
- * they choose the schedule (any values give right results).  O may be Q (same pointer and strides); other overlaps of O
+ * they choose the schedule (any values give right results; a max_q far above a step's new tokens makes it up to twice as slow).  O may be Q (same pointer and strides); other overlaps of O
  * or the workspace with a buffer of the call are refused (DECA_ERR_UNSUPPORTED; _check leaves them to the launch).
  * Strides of Q, K and V are positive (K and V may have a head stride of 0: one key head seen as several).
  * ------------------------------------------------------------------------------------- */

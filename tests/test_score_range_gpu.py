@@ -187,3 +187,19 @@ def test_paged_first_scores_minus_infinity(dead, D, dtype, max_q, max_kv):
             elif at % 3 == 0:
                 set_key(kc, table, 0, at, -199 / 64, 64)
         compare(run_paged(data, 64, max_q, max_kv, 8.0 / D), data, 8.0 / D)
+
+
+@pytest.mark.parametrize("max_q,max_kv", SCHEDULES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_paged_all_scores_minus_infinity(D, max_q, max_kv):
+    """A row without a finite score gives zeros, like one that sees no key; the rows that see one more key do not."""
+    data = make_paged([300], [40], 2, 1, D, 64, torch.float16)
+    q, kc, vc, table, _, _ = data
+    q.fill_(1.0)
+    for at in range(280):
+        set_key(kc, table, 0, at, -math.inf, 64, 5)
+    got = run_paged(data, 64, max_q, max_kv, D**-0.5)
+    assert (got[:20] == 0).all()  # tokens 260 .. 279
+    first = vc[table[0, 280 // 64].long(), 280 % 64, 0]
+    assert torch.equal(got[20], first.expand(2, D))  # one key of weight one
+    assert torch.isfinite(got.float()).all()
