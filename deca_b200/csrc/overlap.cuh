@@ -44,9 +44,9 @@ inline void region_span(const Region &r, int64_t pitch, __int128 *first, __int12
     }
 }
 
-// Whether no byte belongs to both, shown by spans that do not meet (pitch = 0), or by spans of at most one pitch that do
-// not meet on a circle of that length: column blocks of one projection, keys and values that alternate in one cache.
-// False where neither shows it.
+// Whether no byte belongs to both, shown by spans that do not meet (pitch = 0), by spans of at most one pitch that do
+// not meet on a circle of that length (column blocks of one projection, keys and values that alternate in one cache), or
+// block by block where both repeat with one stride that is longer than both together.  False where none shows it.
 inline bool regions_apart(const Region &a, const Region &b) {
     if (region_empty(a) || region_empty(b)) return true;
     auto apart_at = [&](int64_t pitch) {
@@ -64,6 +64,17 @@ inline bool regions_apart(const Region &a, const Region &b) {
         for (int i = 0; i < 4; ++i) {
             const int64_t pitch = r->stride[i] < 0 ? -r->stride[i] : r->stride[i];
             if (r->count[i] > 1 && pitch > 0 && apart_at(pitch)) return true;
+        }
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < 4; ++j) {
+            if (a.count[i] <= 1 || b.count[j] <= 1 || a.stride[i] != b.stride[j] || a.stride[i] <= 0) continue;
+            Region x = a, y = b;
+            x.count[i] = y.count[j] = 1;
+            __int128 x0, xn, y0, yn;
+            region_span(x, 0, &x0, &xn);
+            region_span(y, 0, &y0, &yn);
+            const __int128 from = x0 < y0 ? x0 : y0, to = x0 + xn > y0 + yn ? x0 + xn : y0 + yn;
+            if (to - from <= a.stride[i] && regions_apart(x, y)) return true;
         }
     return false;
 }

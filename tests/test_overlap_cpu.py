@@ -139,3 +139,44 @@ def test_paged_attention_takes(native, kw):
     {"workspace": K}, {"workspace": 2 * K}, {"workspace": 3 * K + 4096}, {"workspace": 4 * K}, {"workspace": 5 * K}, {"workspace": 6 * K}, {"workspace": 7 * K - 256}])
 def test_paged_attention_refuses(native, kw):
     assert attend(native, **kw) == OVERLAP
+
+
+@pytest.mark.parametrize("kw,code", [
+    ({"kc": (5 * K, 4104, 256), "vc": (5 * K + 256, 4104, 256)}, 0),  # rows of keys, then values, in pages with a tail
+    ({"kc": (5 * K, 4104, 256, 128), "vc": (5 * K + 128, 4104, 256, 128)}, 0),
+    ({"kc": (5 * K, 4104, 264, 128), "vc": (5 * K + 128, 4104 + 120, 264, 128)}, OVERLAP),  # other pitches of pages
+    ({"kc": (5 * K, 4352, 264, 128), "vc": (5 * K + 128, 4352, 264, 128)}, 0),  # a tail behind rows and behind pages
+    ({"kc": (5 * K, 4352, 264, 128), "vc": (5 * K + 126, 4352, 264, 128)}, OVERLAP),
+    ({"kc": (5 * K, 4104, 256), "vc": (5 * K + 254, 4104, 256)}, OVERLAP)])
+def test_caches_with_tails(native, kw, code):
+    got = append(native, **kw)
+    assert got == code if code else got not in (0, OVERLAP)
+
+
+def test_regions_against_enumeration(native):
+    """Small layouts of two caches, byte by byte: what shares a byte is always refused; what is accepted shares none."""
+    import random
+
+    rng = random.Random(5)
+    seen = {True: 0, False: 0}
+    for _ in range(4000):
+        def layout():
+            dims = [64 * rng.choice([1, 2, 3, 4]) for _ in range(3)]
+            rng.shuffle(dims)
+            return 5 * K + 64 * rng.randrange(0, 24), tuple(d * rng.choice([1, 1, 2, 5, 16, 33]) for d in dims)
+
+        (k_at, k_strides), (v_at, v_strides) = layout(), layout()
+        if rng.random() < 0.6:
+            v_strides = k_strides
+
+        def bytes_of(at, strides):  # 2 pages x 16 rows x 2 heads, in units of a head's 128 bytes split in two
+            return {at + 2 * (p * strides[0] + r * strides[1] + h * strides[2]) + half for p in range(2) for r in range(16) for h in range(2) for half in (0, 64)}
+
+        def cover(at, strides):
+            return {b // 64 for b in bytes_of(at, strides)}
+
+        share = bool(cover(k_at, k_strides) & cover(v_at, v_strides))
+        refused = append(native, kc=(k_at, *k_strides), vc=(v_at, *v_strides), pages=2) == OVERLAP
+        assert refused or not share, (k_at, k_strides, v_at, v_strides)
+        seen[refused] += 1
+    assert seen[True] > 300 and seen[False] > 300
